@@ -30,6 +30,13 @@ SYMBOLS = (
     "vdb_synth_rows_dev", "vdb_add_synth", "vdb_rebalance", "vdb_warm",
 )
 
+#: every symbol include/vdb_ops.h declares: the encoder operators, in the HIP engine only
+OP_SYMBOLS = (
+    "vdb_op_linear_workspace_bytes", "vdb_op_linear_dev", "vdb_op_linear_backward_workspace_bytes", "vdb_op_linear_backward_dev",
+    "vdb_op_attention_dev", "vdb_op_attention_backward_workspace_bytes", "vdb_op_attention_backward_dev",
+    "vdb_op_mean_pool_dev", "vdb_op_mean_pool_backward_dev",
+)
+
 
 class VdbError(RuntimeError):
     """Raised when a vdb_* call returns a negative status."""
@@ -91,6 +98,23 @@ def _declare(lib: C.CDLL) -> C.CDLL:
     return lib
 
 
+def _declare_ops(lib: C.CDLL) -> C.CDLL:
+    vp, i32, i64, f32 = C.c_void_p, C.c_int, C.c_int64, C.c_float
+    lib.vdb_op_linear_workspace_bytes.argtypes = [i32, i64, i64, i64]
+    lib.vdb_op_linear_dev.argtypes = [i32, i32, vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, i64, i64, i64, i32, vp, i64, vp]
+    lib.vdb_op_linear_backward_workspace_bytes.argtypes = [i32, i64, i64, i64, i32]
+    lib.vdb_op_linear_backward_dev.argtypes = [i32, i32, vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, i64, i64, i64, i32, vp, i64, vp]
+    lib.vdb_op_attention_dev.argtypes = [i32, i32, vp, vp, vp, i64, i64, vp, i32, i32, vp, i64, i64, i32, i32, f32, vp, vp, vp]
+    lib.vdb_op_attention_backward_workspace_bytes.argtypes = [i32, i64, i64, i32, i32, i32]
+    lib.vdb_op_attention_backward_dev.argtypes = [i32, i32, vp, vp, vp, i64, i64, vp, i32, i32, vp, i64, i64, i32, i32, f32, vp, vp, vp,
+                                                  vp, vp, vp, i64, i64, vp, vp, i64, vp]
+    lib.vdb_op_mean_pool_dev.argtypes = [i32, i32, vp, i64, vp, i64, i64, i64, i32, vp, vp, vp]
+    lib.vdb_op_mean_pool_backward_dev.argtypes = [i32, i32, vp, vp, vp, vp, i64, i64, i64, i32, vp, vp]
+    for name in OP_SYMBOLS:
+        getattr(lib, name).restype = i64 if name.endswith("_bytes") else i32
+    return lib
+
+
 _default_lib: Optional[C.CDLL] = None
 
 
@@ -112,7 +136,7 @@ def load_library(path: Optional[str] = None) -> C.CDLL:
                 import torch  # noqa: F401
             except ImportError:
                 pass
-            _default_lib = _declare(C.CDLL(HIP_LIB_PATH))
+            _default_lib = _declare_ops(_declare(C.CDLL(HIP_LIB_PATH)))
         return _default_lib
     return _declare(C.CDLL(path))
 

@@ -19,6 +19,7 @@
 
 #include "../../include/vdb.h"
 #include "launch.h"
+#include "ops.h"
 #include "select.h"
 #include "synth.h"
 #include "probes.h"
@@ -2209,3 +2210,9 @@ int vdb_add_synth(vdb_t* h, int64_t row0, int64_t n, const vdb_synth_spec* spec)
 }
 
 }  // extern "C"
+
+namespace vdbk {
+void set_last_error(const char* msg) {
+  try { g_err = msg; } catch (...) { g_err.clear(); }   // no exception leaves a C entry point
+}
+}  // namespace vdbk
