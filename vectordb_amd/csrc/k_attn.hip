@@ -1,0 +1,104 @@
+// k_attn.hip — launches of the attention operator.
+#include <algorithm>
+#include "op_attn.h"
+
+namespace vdbk {
+namespace {
+
+// Queries (or keys) per block, by the average length, which is all the host knows: 32 rows a wave; a block that is wider
+// than its sequence leaves waves idle, one that is narrower stages the sequence's rows more often.
+int tile_waves(int64_t n_seqs, int64_t total) {
+  const int64_t mean = n_seqs ? total / n_seqs : 0;
+  return mean <= 32 ? 1 : mean <= 64 ? 2 : 4;
+}
+
+AttnParams params(const AttnArgs& a, int elem) {
+  AttnParams p{};
+  p.q = a.q; p.k = a.k; p.v = a.v; p.ld_t = a.ld_t; p.ld_h = a.ld_h; p.table = a.table; p.n_buckets = a.n_buckets;
+  p.offsets = a.offsets; p.n_seqs = a.n_seqs; p.total = a.total; p.heads = a.heads; p.d = a.d; p.scale = a.scale;
+  p.out = a.out; p.lse = a.lse; p.dout = a.dout; p.dq = a.dq; p.dk = a.dk; p.dv = a.dv; p.gld_t = a.gld_t; p.gld_h = a.gld_h;
+  p.bk = a.bk;
+  p.reach = a.bk.n_steps ? a.bk.step[a.bk.n_steps - 1] : a.bk.near;
+  const int64_t v = 16 / elem;
+  auto al = [](const void* x) { return ((uintptr_t)x & 15) == 0; };
+  p.vec = al(a.q) && al(a.k) && al(a.v) && al(a.out) && al(a.dout) && al(a.dq) && al(a.dk) && al(a.dv) && a.d % v == 0 && a.ld_t % v == 0 &&
+          a.ld_h % v == 0 && a.gld_t % v == 0 && a.gld_h % v == 0;
+  return p;
+}
+
+template <typename T, int DP, int NW>
+hipError_t forward(const AttnParams& p, hipStream_t st) {
+  const unsigned grid = (unsigned)(n_slots(p.total, p.n_seqs, NW * 32) * p.heads);
+  attention_kernel<T, DP, NW><<<grid, NW * 64, (2 * p.reach + 1) * sizeof(float), st>>>(p);
+  return hipGetLastError();
+}
+
+template <typename T, int DP, int NW>
+hipError_t backward(const AttnParams& p, const AttnArgs& a) {
+  const int64_t slots = n_slots(p.total, p.n_seqs, NW * 32);
+  const unsigned grid = (unsigned)(slots * p.heads);
+  const size_t line = (2 * p.reach + 1) * sizeof(float), hist = (size_t)NW * 2 * 2 * (p.reach + 64) * sizeof(float);
+  if (a.dtable) attention_dq_kernel<T, DP, NW, true><<<grid, NW * 64, line + hist, a.st>>>(p);
+  else attention_dq_kernel<T, DP, NW, false><<<grid, NW * 64, line, a.st>>>(p);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  attention_dkv_kernel<T, DP, NW><<<grid, NW * 64, line, a.st>>>(p);
+  if ((e = hipGetLastError()) != hipSuccess || !a.dtable) return e;
+  attention_dtable_kernel<T><<<(unsigned)(p.heads * p.n_buckets), 256, 0, a.st>>>(p.part, slots, p.heads, p.n_buckets, (T*)a.dtable);
+  return hipGetLastError();
+}
+
+template <typename T, int DP>
+hipError_t run_dp(const AttnParams& p, const AttnArgs& a, bool back) {
+  switch (tile_waves(p.n_seqs, p.total)) {
+    case 1: return back ? backward<T, DP, 1>(p, a) : forward<T, DP, 1>(p, a.st);
+    case 2: return back ? backward<T, DP, 2>(p, a) : forward<T, DP, 2>(p, a.st);
+    default: return back ? backward<T, DP, 4>(p, a) : forward<T, DP, 4>(p, a.st);
+  }
+}
+
+template <typename T>
+hipError_t run_t(const AttnArgs& a, bool back) {
+  AttnParams p = params(a, sizeof(T));
+  p.delta = a.delta; p.part = a.part; p.peak = (const unsigned*)a.gscale;
+  if (back) {
+    const unsigned grid = (unsigned)(n_slots(p.total, p.n_seqs, 32) * p.heads);
+    if (a.gscale) {
+      const long long n = 2ll * p.heads * p.n_seqs;
+      if (n) fill_zero_kernel<<<(unsigned)std::min<long long>((n + 255) / 256, 1024), 256, 0, a.st>>>((unsigned*)a.gscale, n);
+      attention_delta_kernel<T, true><<<grid, 256, 0, a.st>>>(p, (unsigned*)a.gscale);
+    } else {
+      attention_delta_kernel<T, false><<<grid, 256, 0, a.st>>>(p, nullptr);
+    }
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return p.d <= 32 ? run_dp<T, 32>(p, a, back) : p.d <= 64 ? run_dp<T, 64>(p, a, back) : run_dp<T, 128>(p, a, back);
+}
+
+int64_t pad256(int64_t x) { return (x + 255) / 256 * 256; }
+int64_t part_bytes(int64_t n_seqs, int64_t total, int heads, int n_buckets) {
+  return pad256(n_slots(total, n_seqs, 32 * tile_waves(n_seqs, total)) * heads * n_buckets * 4);
+}
+
+}  // namespace
+
+hipError_t launch_attention(int dtype, const AttnArgs& a) {
+  return dtype == 0 ? run_t<float>(a, false) : dtype == 1 ? run_t<__bf16>(a, false) : run_t<_Float16>(a, false);
+}
+
+int64_t attention_backward_workspace(int dtype, int64_t n_seqs, int64_t total, int heads, int d, int n_buckets) {
+  (void)d;
+  return pad256(total * heads * 4) + (dtype == 2 ? pad256(2 * n_seqs * heads * 4) : 0) + part_bytes(n_seqs, total, heads, n_buckets);
+}
+
+hipError_t launch_attention_backward(int dtype, AttnArgs a, char* ws) {
+  a.delta = (float*)ws;
+  ws += pad256(a.total * a.heads * 4);
+  a.gscale = nullptr;
+  if (dtype == 2) { a.gscale = (float*)ws; ws += pad256(2 * a.n_seqs * a.heads * 4); }
+  a.part = (float*)ws;
+  return dtype == 0 ? run_t<float>(a, true) : dtype == 1 ? run_t<__bf16>(a, true) : run_t<_Float16>(a, true);
+}
+
+}  // namespace vdbk

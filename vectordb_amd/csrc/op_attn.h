@@ -1,0 +1,474 @@
+// op_attn.h — self-attention over packed sequences with a learned relative position bias, forward and backward.
+//
+//   s_ij = scale q_i.k_j + table[bucket(j - i)][h],  p = softmax_j(s),  o_i = sum_j p_ij v_j
+//   ds = p (do v^T - rowsum(do o));  dq = scale ds k,  dk = scale ds^T q,  dv = p^T do,  dtable = bucket sums of ds
+//
+// The bias depends on j - i alone and is constant beyond the last bucket's first distance R, so a block keeps ONE line of
+// 2R + 1 values for its head in LDS (log2 units) instead of any [len][len] matrix; a 32x32 tile wholly beyond R needs no
+// look-up at all.  Softmax runs in base 2 with a running maximum and sum, both fp32.
+//
+// Every product is arranged so that its C registers are the next product's operand (op_common.h): the forward pass and dq
+// compute s^T with the keys in the registers and one query per lane, dk / dv compute s with the queries in the registers.
+#pragma once
+#include "op_common.h"
+#include "ops.h"
+
+namespace vdbk {
+
+struct AttnParams {
+  const void *q, *k, *v; long long ld_t, ld_h;
+  const void* table; int n_buckets;
+  const int64_t* offsets; long long n_seqs, total;
+  int heads, d; float scale;
+  void* out; float* lse;
+  const void* dout; void *dq, *dk, *dv; long long gld_t, gld_h;
+  float* delta; const unsigned* peak; float* part;   // peak: [2][heads][n_seqs] largest |dout| and |v| (fp16 only)
+  int vec;        // q, k, v, out, dout, gradients: 16-byte rows
+  int reach;      // R
+  Buckets bk;
+};
+
+__device__ __forceinline__ int bucket_of(const Buckets& bk, int e) {
+  const int n = e < 0 ? -e : e;
+  int b = n;
+  if (n >= bk.near) {
+    b = bk.near;
+    for (int i = 0; i < bk.n_steps; ++i) b += n >= bk.step[i];
+  }
+  return b + (e > 0 ? bk.half : 0);
+}
+
+// line[R + e] = bias(e) * log2(e) for |e| <= R.  A finite bias stays finite: the product of the type's lowest value with
+// log2(e) would be -inf and a row of such values would lose its softmax.
+template <typename T>
+__device__ __forceinline__ void make_line(float* line, const AttnParams& p, int head) {
+  for (int t = threadIdx.x; t <= 2 * p.reach; t += blockDim.x) {
+    const float b = (float)((const T*)p.table)[(long long)bucket_of(p.bk, t - p.reach) * p.heads + head];
+    float x = b * kLog2e;
+    if (__builtin_isinf(x) && !__builtin_isinf(b)) x = b < 0.f ? -3.4028234e38f : 3.4028234e38f;
+    line[t] = x;
+  }
+}
+
+// ROWS rows of one head into LDS: [ROWS][DP + V], or transposed [DP][ROWS + V]; zeros beyond `valid` rows and d columns.
+template <typename T, int DP, int ROWS, bool PLAIN, bool TRANS>
+__device__ __forceinline__ void stage_rows(T* s, T* st, const T* g, long long ld, int valid, int d, int vec_ok, int threads) {
+  constexpr int V = Elem<T>::kVec;
+  using vec = typename Elem<T>::vec;
+  for (int t = threadIdx.x; t < ROWS * (DP / V); t += threads) {
+    const int r = t / (DP / V), c = (t % (DP / V)) * V;
+    T x[V];
+    if (vec_ok && r < valid && c + V <= d) {
+      *(vec*)x = *(const vec*)(g + r * ld + c);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[e] = r < valid && c + e < d ? g[r * ld + c + e] : (T)0.f;
+    }
+    if constexpr (PLAIN) *(vec*)&s[r * (DP + V) + c] = *(vec*)x;
+    if constexpr (TRANS) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) st[(c + e) * (ROWS + V) + r] = x[e];
+    }
+  }
+}
+
+// One row's operand registers for contractions over the head dimension: piece s holds columns 2 V s + V half ..
+template <typename T, int DP>
+__device__ __forceinline__ void load_row_frags(typename Elem<T>::vec (&f)[DP / (2 * Elem<T>::kVec)], const T* row, bool there, int d, int vec_ok) {
+  constexpr int V = Elem<T>::kVec;
+  using vec = typename Elem<T>::vec;
+  const int half = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int s = 0; s < DP / (2 * V); ++s) {
+    const int c = s * 2 * V + half * V;
+    if (vec_ok && there && c + V <= d) f[s] = *(const vec*)(row + c);
+    else {
+      vec x;
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[e] = there && c + e < d ? row[c + e] : (T)0.f;
+      f[s] = x;
+    }
+  }
+}
+
+// 32 LDS rows (plain layout) times a row operand in registers: C rows = the LDS rows, C column = the lane's row
+template <typename T, int DP>
+__device__ __forceinline__ f32x16 rows_times(const T* s, const typename Elem<T>::vec (&f)[DP / (2 * Elem<T>::kVec)]) {
+  constexpr int V = Elem<T>::kVec;
+  const int lane = threadIdx.x & 63;
+  f32x16 c = {};
+#pragma unroll
+  for (int i = 0; i < DP / (2 * V); ++i)
+    Elem<T>::mma(*(const typename Elem<T>::vec*)&s[(lane & 31) * (DP + V) + i * 2 * V + (lane >> 5) * V], f[i], c);
+  return c;
+}
+
+// acc[db] += X^T p for X = 32 rows in LDS, transposed layout [DP][32 + V], and p a 32x32 tile in C registers (rows = X's rows):
+// C rows = head dimension db * 32 .., C column = p's column.
+template <typename T, int DP>
+__device__ __forceinline__ void trans_times(f32x16 (&acc)[DP / 32], const T* st, const f32x16& p) {
+  constexpr int V = Elem<T>::kVec, LD = 32 + V;
+  using vec = typename Elem<T>::vec;
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  if constexpr (V == 4) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      vec b = {p[4 * g], p[4 * g + 1], p[4 * g + 2], p[4 * g + 3]};
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db) Elem<T>::mma(*(const vec*)&st[(db * 32 + (lane & 31)) * LD + 8 * g + 4 * half], b, acc[db]);
+    }
+  } else {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      vec b;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) b[e] = (T)p[8 * g + e];
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db) {
+        const T* r = &st[(db * 32 + (lane & 31)) * LD + 16 * g + 4 * half];
+        vec a;
+        *(i32x2*)&a = *(const i32x2*)r;
+        *((i32x2*)&a + 1) = *(const i32x2*)(r + 8);
+        Elem<T>::mma(a, b, acc[db]);
+      }
+    }
+  }
+}
+
+// C registers [DP / 32] with C column = a token row: store columns [0, d) of that row, scaled
+template <typename T, int DP>
+__device__ __forceinline__ void store_cols(T* row, const f32x16 (&acc)[DP / 32], float f, int d, int vec_ok) {
+  const int half = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = db * 32 + 8 * g + 4 * half;
+      T x[4] = {(T)(acc[db][4 * g] * f), (T)(acc[db][4 * g + 1] * f), (T)(acc[db][4 * g + 2] * f), (T)(acc[db][4 * g + 3] * f)};
+      if (vec_ok && c + 4 <= d) {
+        if constexpr (sizeof(T) == 2) *(i32x2*)(row + c) = *(i32x2*)x; else *(i32x4*)(row + c) = *(i32x4*)x;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) if (c + e < d) row[c + e] = x[e];
+      }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void zero_rows(T* base, long long ld, long long first, long long last, int d) {
+  const long long n = (last - first) * d;
+  for (long long t = threadIdx.x; t < n; t += blockDim.x) base[(first + t / d) * ld + t % d] = (T)0.f;
+}
+
+// s (fp32 sums) -> log2-unit scores of a 32x32 tile with the keys in the rows and the lane's query as the column, or the
+// other way round; e0 = (first key - first query) of the tile
+template <bool KEYS_IN_ROWS>
+__device__ __forceinline__ void add_bias(f32x16& s, float c, const float* line, int reach, int e0) {
+  const int lane = threadIdx.x & 63;
+  if (e0 - 31 >= reach || e0 + 31 <= -reach) {
+    const float b = line[e0 > 0 ? 2 * reach : 0];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = s[r] * c + b;
+    return;
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int row = (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5), col = lane & 31;
+    int e = e0 + (KEYS_IN_ROWS ? row - col : col - row);
+    e = e > reach ? reach : e < -reach ? -reach : e;
+    s[r] = s[r] * c + line[reach + e];
+  }
+}
+
+// ---- forward ------------------------------------------------------------------------------------------------------------
+// Block: one slot of NW * 32 queries of one head; each wave 32 queries, one per lane column; key tiles of 32 through LDS.
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64) void attention_kernel(const AttnParams p) {
+  constexpr int V = Elem<T>::kVec, BQ = NW * 32;
+  __shared__ __align__(16) T sk[32 * (DP + V)];
+  __shared__ __align__(16) T sv[DP * (32 + V)];
+  extern __shared__ float line[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int head = blockIdx.x % p.heads;
+  const Slot s = find_slot(p.offsets, p.n_seqs, p.total, BQ, blockIdx.x / p.heads);
+  if (s.b < 0) return;
+  const long long hd = (long long)p.heads * p.d;
+  if (s.b == p.n_seqs) {
+    const long long r0 = s.begin + (long long)s.tile * BQ, r1 = r0 + BQ < s.end ? r0 + BQ : s.end;
+    zero_rows((T*)p.out + (long long)head * p.d, hd, r0, r1, p.d);
+    return;
+  }
+  const int len = (int)(s.end - s.begin);
+  const int i0 = s.tile * BQ + wave * 32, i = i0 + (lane & 31);
+  make_line<T>(line, p, head);
+  const T* kb = (const T*)p.k + s.begin * p.ld_t + head * p.ld_h;
+  const T* vb = (const T*)p.v + s.begin * p.ld_t + head * p.ld_h;
+  typename Elem<T>::vec fq[DP / (2 * V)];
+  load_row_frags<T, DP>(fq, (const T*)p.q + (s.begin + i) * p.ld_t + head * p.ld_h, i < len, p.d, p.vec);
+  const float c = p.scale * kLog2e;
+  float m = -INFINITY, l = 0.f;
+  f32x16 acc[DP / 32] = {};
+  for (int j0 = 0; j0 < len; j0 += 32) {
+    __syncthreads();
+    stage_rows<T, DP, 32, true, false>(sk, nullptr, kb + j0 * p.ld_t, p.ld_t, len - j0, p.d, p.vec, NW * 64);
+    stage_rows<T, DP, 32, false, true>(nullptr, sv, vb + j0 * p.ld_t, p.ld_t, len - j0, p.d, p.vec, NW * 64);
+    __syncthreads();
+    if (i0 >= len) continue;
+    f32x16 t = rows_times<T, DP>(sk, fq);
+    add_bias<true>(t, c, line, p.reach, j0 - i0);
+    if (j0 + 32 > len) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) if (j0 + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5) >= len) t[r] = -INFINITY;
+    }
+    float top = t[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) top = fmaxf(top, t[r]);
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const float m1 = fmaxf(m, top), ms = m1 == -INFINITY ? 0.f : m1;   // a row of -inf alone: p = 0, not NaN
+    const float fade = exp2f(m - ms);
+    l *= fade;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) { t[r] = exp2f(t[r] - ms); l += t[r]; }
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) acc[db] *= fade;
+    trans_times<T, DP>(acc, sv, t);
+    m = m1;
+  }
+  if (i >= len) return;
+  l += __shfl_xor(l, 32, 64);
+  store_cols<T, DP>((T*)p.out + (s.begin + i) * hd + (long long)head * p.d, acc, l > 0.f || l != l ? 1.f / l : 0.f, p.d, p.vec);
+  // +inf where nothing was left of the row: the backward pass' exp2(s - lse) is 0 there
+  if (p.lse && lane < 32) p.lse[(long long)head * p.total + s.begin + i] = l > 0.f || l != l ? m + log2f(l) : INFINITY;
+}
+
+// ---- backward -------------------------------------------------------------------------------------------------------------
+// delta[h][t] = sum_d dout out; fp16 also the largest |dout| and |v| of each sequence and head (bits of non-negative
+// floats order like integers, so the atomic maximum does not depend on the order of arrival).
+template <typename T, bool PEAK>
+__global__ __launch_bounds__(256) void attention_delta_kernel(const AttnParams p, unsigned* peak) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int head = blockIdx.x % p.heads;
+  const Slot s = find_slot(p.offsets, p.n_seqs, p.total, 32, blockIdx.x / p.heads);
+  if (s.b < 0 || s.b == p.n_seqs) return;
+  float po = 0.f, pv = 0.f;
+  for (int r = wave; r < 32; r += 4) {
+    const long long t = s.begin + (long long)s.tile * 32 + r;
+    if (t >= s.end) break;
+    const T* o = (const T*)p.out + (t * p.heads + head) * p.d;
+    const T* g = (const T*)p.dout + (t * p.heads + head) * p.d;
+    const T* v = (const T*)p.v + t * p.ld_t + head * p.ld_h;
+    float x = 0.f;
+    for (int c = lane; c < p.d; c += 64) {
+      x += (float)o[c] * (float)g[c];
+      if (PEAK) { po = fmaxf(po, fabsf((float)g[c])); pv = fmaxf(pv, fabsf((float)v[c])); }
+    }
+    for (int k = 32; k; k >>= 1) x += __shfl_xor(x, k, 64);
+    if (lane == 0) p.delta[(long long)head * p.total + t] = x;
+  }
+  if (PEAK) {
+    for (int k = 32; k; k >>= 1) { po = fmaxf(po, __shfl_xor(po, k, 64)); pv = fmaxf(pv, __shfl_xor(pv, k, 64)); }
+    if (lane == 0) {
+      atomicMax(peak + (long long)head * p.n_seqs + s.b, __float_as_uint(po));
+      atomicMax(peak + ((long long)p.heads + head) * p.n_seqs + s.b, __float_as_uint(pv));
+    }
+  }
+}
+
+static __global__ void fill_zero_kernel(unsigned* x, long long n) {
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) x[i] = 0;
+}
+
+// fp16 has five exponent bits: ds of a long row (p ~ 1 / len) times a small gradient would fall among its subnormals.
+// A power of two per sequence and head lifts it: |ds| <= 2 d max|dout| max|v| stays below 2^15.
+template <typename T>
+__device__ __forceinline__ float ds_lift(const AttnParams& p, int head, long long b) {
+  if constexpr (sizeof(T) == 2 && !__is_same(T, __bf16)) {
+    const float po = __uint_as_float(p.peak[(long long)head * p.n_seqs + b]), pv = __uint_as_float(p.peak[((long long)p.heads + head) * p.n_seqs + b]);
+    const float bound = 2.f * (float)p.d * po * pv;
+    if (!(bound > 0.f) || bound > 1e30f || bound < 1e-30f) return 1.f;
+    return exp2f((float)(14 - ilogbf(bound)));
+  } else {
+    return 1.f;
+  }
+}
+
+// dq and the block's part of dtable: like the forward pass, with ds^T in the place of p^T.
+// The bucket sums: each half of a wave adds its tile's ds by distance into a line of its own in LDS.  The additions are LDS
+// atomics only because lanes meet at an address in DIFFERENT instructions: the 32 lanes of a half hold 32 different distances
+// at every step, and a wave's LDS operations keep their order, so nothing depends on timing.  Tiles beyond R go into two
+// registers.  One thread per bucket then adds up its distances, in order.
+template <typename T, int DP, int NW, bool DTABLE>
+__global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnParams p) {
+  constexpr int V = Elem<T>::kVec, BQ = NW * 32;
+  __shared__ __align__(16) T sk[32 * (DP + V)];
+  __shared__ __align__(16) T skt[DP * (32 + V)];
+  __shared__ __align__(16) T sv[32 * (DP + V)];
+  __shared__ float far[NW][2];
+  extern __shared__ float line[];                      // 2R + 1, then NW * 2 lines of 2 (R + 64)
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  const int head = blockIdx.x % p.heads;
+  const long long slot = blockIdx.x / p.heads;
+  const Slot s = find_slot(p.offsets, p.n_seqs, p.total, BQ, slot);
+  float* part = p.part + (slot * p.heads + head) * p.n_buckets;
+  if (s.b < 0 || s.b == p.n_seqs) {
+    if (s.b >= 0) {
+      const long long r0 = s.begin + (long long)s.tile * BQ, r1 = r0 + BQ < s.end ? r0 + BQ : s.end;
+      zero_rows((T*)p.dq + head * p.gld_h, p.gld_t, r0, r1, p.d);
+    }
+    if constexpr (DTABLE) for (int t = threadIdx.x; t < p.n_buckets; t += NW * 64) part[t] = 0.f;
+    return;
+  }
+  const int len = (int)(s.end - s.begin);
+  const int i0 = s.tile * BQ + wave * 32, i = i0 + (lane & 31);
+  const int reach = p.reach, span = 2 * (reach + 64);
+  float* hist = line + 2 * reach + 1;
+  make_line<T>(line, p, head);
+  if constexpr (DTABLE) for (int t = threadIdx.x; t < NW * 2 * span; t += NW * 64) hist[t] = 0.f;
+  float* mine = hist + (wave * 2 + half) * span + reach + 64;   // mine[e]
+  const T* kb = (const T*)p.k + s.begin * p.ld_t + head * p.ld_h;
+  const T* vb = (const T*)p.v + s.begin * p.ld_t + head * p.ld_h;
+  const long long hd = (long long)p.heads * p.d;
+  typename Elem<T>::vec fq[DP / (2 * V)], fg[DP / (2 * V)];
+  load_row_frags<T, DP>(fq, (const T*)p.q + (s.begin + i) * p.ld_t + head * p.ld_h, i < len, p.d, p.vec);
+  load_row_frags<T, DP>(fg, (const T*)p.dout + (s.begin + i) * hd + (long long)head * p.d, i < len, p.d, p.vec);
+  const float lse = i < len ? p.lse[(long long)head * p.total + s.begin + i] : INFINITY;
+  const float delta = i < len ? p.delta[(long long)head * p.total + s.begin + i] : 0.f;
+  const float lift = ds_lift<T>(p, head, s.b);
+  const float c = p.scale * kLog2e;
+  float below = 0.f, above = 0.f;
+  f32x16 acc[DP / 32] = {};
+  for (int j0 = 0; j0 < len; j0 += 32) {
+    __syncthreads();
+    stage_rows<T, DP, 32, true, true>(sk, skt, kb + j0 * p.ld_t, p.ld_t, len - j0, p.d, p.vec, NW * 64);
+    stage_rows<T, DP, 32, true, false>(sv, nullptr, vb + j0 * p.ld_t, p.ld_t, len - j0, p.d, p.vec, NW * 64);
+    __syncthreads();
+    if (i0 >= len) continue;
+    f32x16 t = rows_times<T, DP>(sk, fq);
+    const f32x16 dp = rows_times<T, DP>(sv, fg);
+    const int e0 = j0 - i0;
+    add_bias<true>(t, c, line, reach, e0);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int j = j0 + (r & 3) + 8 * (r >> 2) + 4 * half;
+      const float w = j < len ? exp2f(t[r] - lse) : 0.f;
+      t[r] = w == 0.f ? 0.f : w * (dp[r] - delta);
+    }
+    if constexpr (DTABLE) {
+      if (e0 - 31 >= reach || e0 + 31 <= -reach) {
+        float x = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x += t[r];
+        if (e0 > 0) above += x; else below += x;
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int e = e0 + (r & 3) + 8 * (r >> 2) + 4 * half - (lane & 31);
+          __hip_atomic_fetch_add(mine + e, t[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+        }
+      }
+    }
+    if (lift != 1.f) t *= lift;
+    trans_times<T, DP>(acc, skt, t);
+  }
+  if (i < len) store_cols<T, DP>((T*)p.dq + (s.begin + i) * p.gld_t + head * p.gld_h, acc, p.scale / lift, p.d, p.vec);
+  if constexpr (DTABLE) {
+    for (int k = 32; k; k >>= 1) { below += __shfl_xor(below, k, 64); above += __shfl_xor(above, k, 64); }
+    if (lane == 0) { far[wave][0] = below; far[wave][1] = above; }
+    __syncthreads();
+    for (int t = threadIdx.x; t < p.n_buckets; t += NW * 64) {
+      const int low = t % p.bk.half, side = t / p.bk.half;        // t < 2 half
+      const int n0 = low <= p.bk.near ? low : p.bk.step[low - p.bk.near - 1];
+      const int n1 = low + 1 == p.bk.half ? reach + 64 : low + 1 <= p.bk.near ? low + 1 : p.bk.step[low - p.bk.near];
+      float x = 0.f;
+      for (int w = 0; w < NW; ++w) {
+        if (low + 1 == p.bk.half) x += far[w][side];
+        for (int g = 0; g < 2; ++g) {
+          const float* h = hist + (w * 2 + g) * span + reach + 64;
+          for (int n = side ? (n0 > 1 ? n0 : 1) : n0; n < n1; ++n) x += h[side ? n : -n];
+        }
+      }
+      part[t] = x;
+    }
+  }
+}
+
+// dk and dv: block = NW * 32 keys of one head, one key per lane column; query tiles of 32 through LDS.
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64) void attention_dkv_kernel(const AttnParams p) {
+  constexpr int V = Elem<T>::kVec, BQ = NW * 32;
+  __shared__ __align__(16) T sq[32 * (DP + V)];
+  __shared__ __align__(16) T sqt[DP * (32 + V)];
+  __shared__ __align__(16) T sg[32 * (DP + V)];
+  __shared__ __align__(16) T sgt[DP * (32 + V)];
+  __shared__ __align__(16) float sl[32], sd[32];
+  extern __shared__ float line[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  const int head = blockIdx.x % p.heads;
+  const Slot s = find_slot(p.offsets, p.n_seqs, p.total, BQ, blockIdx.x / p.heads);
+  if (s.b < 0) return;
+  if (s.b == p.n_seqs) {
+    const long long r0 = s.begin + (long long)s.tile * BQ, r1 = r0 + BQ < s.end ? r0 + BQ : s.end;
+    zero_rows((T*)p.dk + head * p.gld_h, p.gld_t, r0, r1, p.d);
+    zero_rows((T*)p.dv + head * p.gld_h, p.gld_t, r0, r1, p.d);
+    return;
+  }
+  const int len = (int)(s.end - s.begin);
+  const int j0 = s.tile * BQ + wave * 32, j = j0 + (lane & 31);
+  make_line<T>(line, p, head);
+  const long long hd = (long long)p.heads * p.d;
+  typename Elem<T>::vec fk[DP / (2 * V)], fv[DP / (2 * V)];
+  load_row_frags<T, DP>(fk, (const T*)p.k + (s.begin + j) * p.ld_t + head * p.ld_h, j < len, p.d, p.vec);
+  load_row_frags<T, DP>(fv, (const T*)p.v + (s.begin + j) * p.ld_t + head * p.ld_h, j < len, p.d, p.vec);
+  const T* qb = (const T*)p.q + s.begin * p.ld_t + head * p.ld_h;
+  const T* gb = (const T*)p.dout + s.begin * hd + (long long)head * p.d;
+  const float* lse = p.lse + (long long)head * p.total + s.begin;
+  const float* delta = p.delta + (long long)head * p.total + s.begin;
+  const float lift = ds_lift<T>(p, head, s.b);
+  const float c = p.scale * kLog2e;
+  f32x16 ak[DP / 32] = {}, av[DP / 32] = {};
+  for (int i0 = 0; i0 < len; i0 += 32) {
+    __syncthreads();
+    stage_rows<T, DP, 32, true, true>(sq, sqt, qb + i0 * p.ld_t, p.ld_t, len - i0, p.d, p.vec, NW * 64);
+    stage_rows<T, DP, 32, true, true>(sg, sgt, gb + i0 * hd, hd, len - i0, p.d, p.vec, NW * 64);
+    if (threadIdx.x < 32) {
+      sl[threadIdx.x] = i0 + (int)threadIdx.x < len ? lse[i0 + threadIdx.x] : INFINITY;
+      sd[threadIdx.x] = i0 + (int)threadIdx.x < len ? delta[i0 + threadIdx.x] : 0.f;
+    }
+    __syncthreads();
+    if (j0 >= len) continue;
+    f32x16 t = rows_times<T, DP>(sq, fk);
+    const f32x16 dp = rows_times<T, DP>(sg, fv);
+    add_bias<false>(t, c, line, p.reach, j0 - i0);
+    f32x16 ds;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int row = (r & 3) + 8 * (r >> 2) + 4 * half;
+      t[r] = exp2f(t[r] - sl[row]);
+      ds[r] = t[r] == 0.f ? 0.f : t[r] * (dp[r] - sd[row]);
+    }
+    trans_times<T, DP>(av, sgt, t);
+    if (lift != 1.f) ds *= lift;
+    trans_times<T, DP>(ak, sqt, ds);
+  }
+  if (j >= len) return;
+  store_cols<T, DP>((T*)p.dk + (s.begin + j) * p.gld_t + head * p.gld_h, ak, p.scale / lift, p.d, p.vec);
+  store_cols<T, DP>((T*)p.dv + (s.begin + j) * p.gld_t + head * p.gld_h, av, 1.f, p.d, p.vec);
+}
+
+// dtable[t][h] = the slots' parts in order, in 64 bits: block = one head and bucket
+template <typename T>
+__global__ __launch_bounds__(256) void attention_dtable_kernel(const float* __restrict__ part, long long slots, int heads, int n_buckets, T* __restrict__ dtable) {
+  __shared__ double red[256];
+  const int t = blockIdx.x % n_buckets, head = blockIdx.x / n_buckets;
+  double x = 0.0;
+  for (long long s = threadIdx.x; s < slots; s += 256) x += part[(s * heads + head) * n_buckets + t];
+  red[threadIdx.x] = x;
+  __syncthreads();
+  for (int k = 128; k; k >>= 1) {
+    if ((int)threadIdx.x < k) red[threadIdx.x] += red[threadIdx.x + k];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) dtable[(long long)t * heads + head] = (T)(float)red[0];
+}
+
+}  // namespace vdbk
