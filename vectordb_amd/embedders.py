@@ -6,7 +6,8 @@ possible offline, so the seam accepts:
 
   * any callable(list[str]) -> array-like [n, dim];
   * MPNetEmbedder(local_dir): transformers MPNet + mean pooling + L2 normalise
-    on PyTorch-ROCm, from a user-supplied local checkpoint directory;
+    on PyTorch-ROCm, from a user-supplied local checkpoint directory; with
+    engine="hip" its layers run on the framework's own operators (ops.py);
   * HashEmbedder: deterministic hashed character-n-gram embedding used by tests
     and demos (NOT semantically equivalent to MPNet).
 """
@@ -52,9 +53,12 @@ class MPNetEmbedder:
     tokenizer + MPNetModel -> attention-masked mean pooling -> L2 normalise."""
 
     def __init__(self, local_dir: str, device: str = None, batch_size: int = 64, max_length: int = 384,
-                 autocast: str = None):
+                 autocast: str = None, engine: str = "transformers"):
         """autocast: None (fp32 forward, the reference's precision), "bf16" or "fp16" (GPU only; the
-        pooled vector is still accumulated and normalised in fp32)."""
+        pooled vector is still accumulated and normalised in fp32).  engine: "transformers" (its
+        forward pass over padded batches) or "hip" (GPU only: encoder.MPNetEncoder on the framework's
+        operators, tokens packed without padding; the same vectors up to rounding, and
+        encode(), which is differentiable)."""
         import torch
         from transformers import AutoModel, AutoTokenizer
         if not os.path.isdir(local_dir):
@@ -69,6 +73,22 @@ class MPNetEmbedder:
             raise ValueError("autocast must be None, 'bf16' or 'fp16'")
         self._amp = {None: None, "bf16": torch.bfloat16, "fp16": torch.float16}[autocast]
         self.dim = int(self.model.config.hidden_size)
+        if engine not in ("transformers", "hip"):
+            raise ValueError("engine must be 'transformers' or 'hip'")
+        self._hip = None
+        if engine == "hip":
+            if not str(self.device).startswith("cuda"):
+                raise ValueError(f"engine='hip' needs a GPU device; got {self.device}")
+            from .encoder import MPNetEncoder
+            self._hip = MPNetEncoder(self.model, self._amp or torch.float32)
+
+    def encode(self, texts: Sequence[str]):
+        """-> torch.Tensor [n, dim] fp32, unit rows, differentiable in self.model's parameters where gradients are
+        enabled (engine="hip"): what fine-tuning on matched products steps through.  All texts as one batch; no dropout."""
+        if self._hip is None:
+            raise ValueError("encode() needs engine='hip'")
+        tokens = self.tok(list(texts), padding=False, truncation=True, max_length=self.max_length)["input_ids"] if len(texts) else []
+        return self._hip.encode(*self._hip.pack(tokens, self.device))
 
     def embed_device(self, texts: Sequence[str]):
         """-> torch.Tensor [n, dim] fp32 on self.device, rows unit length.  On a GPU the result can go
@@ -80,6 +100,9 @@ class MPNetEmbedder:
         dev_type = "cuda" if str(self.device).startswith("cuda") else "cpu"
         with torch.no_grad():
             for i in range(0, len(texts), self.batch_size):
+                if self._hip is not None:
+                    out[i:i + self.batch_size] = self.encode(texts[i:i + self.batch_size])
+                    continue
                 enc = self.tok(texts[i:i + self.batch_size], padding=True, truncation=True,
                                max_length=self.max_length, return_tensors="pt").to(self.device)
                 with torch.autocast(dev_type, dtype=self._amp, enabled=self._amp is not None and dev_type == "cuda"):
@@ -93,15 +116,16 @@ class MPNetEmbedder:
         return list(self.embed_device(texts).cpu().numpy())
 
 
-def SentenceTransformerEmbeddingFunction(model_name: str = "all-mpnet-base-v2", **_ignored):
+def SentenceTransformerEmbeddingFunction(model_name: str = "all-mpnet-base-v2", engine: str = None, **_ignored):
     """Same name and call shape as chromadb.utils.embedding_functions' class, so that
     `from vectordb_amd import embedders as embedding_functions` leaves the reference's
     `src/vectordb.py:17` unchanged.  Resolves offline only (see resolve_embedder)."""
-    return resolve_embedder(model_name)
+    return resolve_embedder(model_name, engine=engine)
 
 
-def resolve_embedder(model_name: str, embed_fn: Callable = None):
-    """embed_fn wins; a local directory -> MPNetEmbedder; 'hash'/'hash:<dim>' -> HashEmbedder."""
+def resolve_embedder(model_name: str, embed_fn: Callable = None, engine: str = None):
+    """embed_fn wins; a local directory -> MPNetEmbedder; 'hash'/'hash:<dim>' -> HashEmbedder.
+    engine: MPNetEmbedder's (default: VECTORDB_EMBED_ENGINE, else "transformers")."""
     if embed_fn is not None:
         return embed_fn
     if isinstance(model_name, str) and model_name.startswith("hash"):
@@ -109,7 +133,7 @@ def resolve_embedder(model_name: str, embed_fn: Callable = None):
         return HashEmbedder(dim)
     local = os.environ.get("VECTORDB_MODEL_DIR", model_name)
     if isinstance(local, str) and os.path.isdir(local):
-        return MPNetEmbedder(local)
+        return MPNetEmbedder(local, engine=engine or os.environ.get("VECTORDB_EMBED_ENGINE") or "transformers")
     raise RuntimeError(
         f"embedding model {model_name!r} is not available offline: pass embed_fn=..., set VECTORDB_MODEL_DIR to a local "
         "checkpoint directory, or use embedding_model_name='hash' for the deterministic test embedder")
