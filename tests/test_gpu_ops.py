@@ -30,7 +30,7 @@ def rnd(g, *shape, dtype=torch.float32, scale=1.0):
 def hold(got, want, what=""):
     """|got - exact| <= bound everywhere."""
     for i, (t, (exact, bound)) in enumerate(zip(got, want)):
-        t = t.detach().cpu().double()
+        t = t.detach().to(exact.device).double()
         assert t.shape == exact.shape, (what, i, t.shape, exact.shape)
         assert torch.isfinite(t).all(), (what, i, "not finite")
         off = (t - exact).abs()
@@ -82,6 +82,35 @@ def test_linear_gradients(ops, dtype, name, m, n, k):
         only = [t.detach().requires_grad_(j == i) for j, t in enumerate(leaves)]
         one, = torch.autograd.grad(ops.linear(only[0], only[1], only[2], name, only[3]), [only[i]], dy.cuda())
         assert torch.equal(one, grads[i])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k,name", [(1000, 776, 776, "none"), (2049, 1400, 72, "gelu"), (8200, 4104, 72, "none"), (8200, 4104, 136, "gelu_tanh"), (2100, 1409, 200, "relu"),
+                                        (16385, 2056, 64, "gelu"), (5000, 40, 1000, "none")])
+def test_linear_forward_large(ops, dtype, m, n, k, name):
+    """Sizes that take each of the tiled kernels, with ragged edges in all three dimensions (64-bit form on the GPU)."""
+    g = torch.Generator(device="cuda").manual_seed(m + n + k)
+    x, w = (torch.randn(*s, generator=g, device="cuda").to(DT[dtype]) for s in ((m, k), (n, k)))
+    b, r = (torch.randn(*s, generator=g, device="cuda").to(DT[dtype]) for s in ((n,), (m, n)))
+    w = w * k ** -0.5
+    hold([ops.linear(x, w, b, name, r)], ref.linear(x, w, b, name, r), dtype)
+    hold([ops.linear(x, w)], ref.linear(x, w, None, "none", None), dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k,name", [(8192, 512, 384, "gelu"), (6001, 264, 776, "none"), (20000, 136, 136, "gelu_tanh"), (4096, 1408, 1416, "none"), (3000, 33, 520, "gelu")])
+def test_linear_gradients_large(ops, dtype, m, n, k, name):
+    """Long contractions that are split over blocks and joined, and their ragged ends."""
+    g = torch.Generator(device="cuda").manual_seed(m + n + k)
+    x, w, b, dy = (torch.randn(*s, generator=g, device="cuda").to(DT[dtype]) for s in ((m, k), (n, k), (n,), (m, n)))
+    w = w * k ** -0.5
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = ops.linear(x, w, b, name)
+    grads = torch.autograd.grad(y, leaves, dy)
+    with torch.no_grad():
+        hold([y, *grads], ref.linear(x, w, b, name, None, dy), dtype)
+    again = torch.autograd.grad(ops.linear(x, w, b, name), leaves, dy)
+    assert all(torch.equal(p, q) for p, q in zip(grads, again))
 
 
 def test_linear_layouts_strides_and_alignment(ops):

@@ -18,7 +18,7 @@ struct GemmArgs {
   float* partial; int64_t partial_bytes;   // scratch for a contraction split over blocks
   hipStream_t st;
 };
-int64_t gemm_workspace_bytes(int dtype, int64_t m, int64_t n, int64_t k);
+int64_t gemm_workspace_bytes(int dtype, bool a_t, bool b_t, int64_t m, int64_t n, int64_t k);
 hipError_t launch_gemm(int dtype, const GemmArgs& a);
 
 // dz = dy act'(z) (dz dense [m][n]; skipped when act is none) and db = column sums of dy act'(z)

@@ -102,7 +102,7 @@ extern "C" {
 
 int64_t vdb_op_linear_workspace_bytes(int dtype, int64_t m, int64_t n, int64_t k) {
   if (!known(dtype) || !widths(m, n, k)) return 0;
-  return gemm_workspace_bytes(dtype, m, n, k);
+  return gemm_workspace_bytes(dtype, false, false, m, n, k);
 }
 
 int vdb_op_linear_dev(int device, int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual,
@@ -114,8 +114,8 @@ int vdb_op_linear_dev(int device, int dtype, const void* x, int64_t ldx, const v
   if (m == 0) return VDB_OK;
   NEED(x && w && y, "linear: a pointer is NULL");
   NEED(ldx >= k && ldw >= k && ldy >= n && (!residual || ldr >= n), "linear: a row stride is smaller than its row");
-  NEED(workspace_bytes >= gemm_workspace_bytes(dtype, m, n, k), "linear: the workspace is too small");
-  NEED(workspace || gemm_workspace_bytes(dtype, m, n, k) == 0, "linear: the workspace is NULL");
+  NEED(workspace_bytes >= gemm_workspace_bytes(dtype, false, false, m, n, k), "linear: the workspace is too small");
+  NEED(workspace || gemm_workspace_bytes(dtype, false, false, m, n, k) == 0, "linear: the workspace is NULL");
   ON_DEVICE("linear");
   GemmArgs a{};
   a.a = x; a.lda = ldx; a.b = w; a.ldb = ldw; a.m = m; a.n = n; a.k = k; a.y = y; a.ldy = ldy; a.bias = bias; a.act = act;
@@ -128,7 +128,7 @@ int vdb_op_linear_dev(int device, int dtype, const void* x, int64_t ldx, const v
 static void backward_pieces(int dtype, int64_t m, int64_t n, int64_t k, int act, int64_t* dz, int64_t* cols, int64_t* split) {
   *dz = act == VDB_ACT_NONE ? 0 : pad256(m * n * elem_size(dtype));
   *cols = pad256((int64_t)act_grad_parts(m, n) * n * 4);
-  const int64_t s1 = gemm_workspace_bytes(dtype, m, k, n), s2 = gemm_workspace_bytes(dtype, n, k, m);
+  const int64_t s1 = gemm_workspace_bytes(dtype, false, true, m, k, n), s2 = gemm_workspace_bytes(dtype, true, true, n, k, m);
   *split = s1 > s2 ? s1 : s2;
 }
 
