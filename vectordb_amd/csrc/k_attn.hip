@@ -22,14 +22,18 @@ AttnParams params(const AttnArgs& a, int elem) {
   const int64_t v = 16 / elem;
   auto al = [](const void* x) { return ((uintptr_t)x & 15) == 0; };
   p.vec = al(a.q) && al(a.k) && al(a.v) && al(a.out) && al(a.dout) && al(a.dq) && al(a.dk) && al(a.dv) && a.d % v == 0 && a.ld_t % v == 0 &&
-          a.ld_h % v == 0 && a.gld_t % v == 0 && a.gld_h % v == 0;
+          a.ld_h % v == 0 && a.gld_t % v == 0 && a.gld_h % v == 0 && a.ld_t < ((int64_t)1 << 22);
   return p;
 }
 
 template <typename T, int DP, int NW>
 hipError_t forward(const AttnParams& p, hipStream_t st) {
-  const unsigned grid = (unsigned)(n_slots(p.total, p.n_seqs, NW * 32) * p.heads);
-  attention_kernel<T, DP, NW><<<grid, NW * 64, (2 * p.reach + 1) * sizeof(float), st>>>(p);
+  const unsigned slots = (unsigned)n_slots(p.total, p.n_seqs, NW * 32), grid = slots * p.heads;
+  if (p.vec && p.d == DP) {
+    attention_kernel<T, DP, NW><<<grid, NW * 64, (2 * (p.reach + kMargin) + 1) * sizeof(float), st>>>(p, slots);
+    return hipGetLastError();
+  }
+  attention_any_kernel<T, DP, NW><<<grid, NW * 64, (2 * p.reach + 1) * sizeof(float), st>>>(p);
   return hipGetLastError();
 }
 

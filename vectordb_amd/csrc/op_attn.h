@@ -180,10 +180,10 @@ __device__ __forceinline__ void add_bias(f32x16& s, float c, const float* line, 
   }
 }
 
-// ---- forward ------------------------------------------------------------------------------------------------------------
+// ---- forward, any width, stride and alignment ---------------------------------------------------------------------------
 // Block: one slot of NW * 32 queries of one head; each wave 32 queries, one per lane column; key tiles of 32 through LDS.
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64) void attention_kernel(const AttnParams p) {
+__global__ __launch_bounds__(NW * 64) void attention_any_kernel(const AttnParams p) {
   constexpr int V = Elem<T>::kVec, BQ = NW * 32;
   __shared__ __align__(16) T sk[32 * (DP + V)];
   __shared__ __align__(16) T sv[DP * (32 + V)];
@@ -225,10 +225,10 @@ __global__ __launch_bounds__(NW * 64) void attention_kernel(const AttnParams p) 
     for (int r = 1; r < 16; ++r) top = fmaxf(top, t[r]);
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     const float m1 = fmaxf(m, top), ms = m1 == -INFINITY ? 0.f : m1;   // a row of -inf alone: p = 0, not NaN
-    const float fade = exp2f(m - ms);
+    const float fade = __builtin_amdgcn_exp2f(m - ms);
     l *= fade;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) { t[r] = exp2f(t[r] - ms); l += t[r]; }
+    for (int r = 0; r < 16; ++r) { t[r] = __builtin_amdgcn_exp2f(t[r] - ms); l += t[r]; }
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) acc[db] *= fade;
     trans_times<T, DP>(acc, sv, t);
@@ -239,6 +239,217 @@ __global__ __launch_bounds__(NW * 64) void attention_kernel(const AttnParams p) 
   store_cols<T, DP>((T*)p.out + (s.begin + i) * hd + (long long)head * p.d, acc, l > 0.f || l != l ? 1.f / l : 0.f, p.d, p.vec);
   // +inf where nothing was left of the row: the backward pass' exp2(s - lse) is 0 there
   if (p.lse && lane < 32) p.lse[(long long)head * p.total + s.begin + i] = l > 0.f || l != l ? m + log2f(l) : INFINITY;
+}
+
+// ---- whole 16-byte pieces and head widths of 32, 64 and 128 ----------------------------------------------------------------
+// Rows of one head in LDS: D values, 16-byte pieces, moved by XOR.  For reads along the row (kRow: 32 rows x 16 bytes at one place)
+// the row number spreads the pieces over all banks; for transposed reads (kCol: 4 rows x 64 bytes, or fp32 words of rows 4 apart)
+// it moves whole 64- or 128-byte groups.
+enum Order { kRow, kCol };
+template <typename T, int D, Order O> struct Rows {
+  static constexpr int V = Elem<T>::kVec, C = D / V;        // pieces of a row
+  using vec = typename Elem<T>::vec;
+  static __device__ __forceinline__ int swz(int row) {
+    if constexpr (O == kRow) return C >= 16 ? row & 15 : C == 8 ? (row >> 1) & 7 : (row >> 2) & 3;
+    else if constexpr (sizeof(T) == 4) return C >= 16 ? (row >> 2 & 1) << 3 : 0;
+    else return C >= 16 ? (row & 3) << 2 : C == 8 ? (row >> 1 & 1) << 2 : 0;
+  }
+  // operand piece i (of D / 2V) for contractions over D: row r0 + lane & 31, r0 a multiple of 32
+  static __device__ __forceinline__ vec along(const T* s, int r0, int i) {
+    const int lane = threadIdx.x & 63, l = lane & 31;
+    return *(const vec*)(s + (r0 + l) * D + (((2 * i + (lane >> 5)) ^ swz(l)) * V));
+  }
+  // operand for contractions over 4 V rows from r0 in the order of C registers, columns c0 + lane & 31
+  static __device__ __forceinline__ vec across(const T* s, int r0, int c0) {
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    vec x;
+    if constexpr (sizeof(T) == 4) {
+      const int l = lane & 31;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = 4 * half + e;                        // r0 is a multiple of 8
+        x[e] = s[(r0 + row) * D + ((((c0 + l) >> 2) ^ swz(row)) << 2) + (l & 3)];
+      }
+    } else {
+      const int i = lane & 15, row = 4 * half + (i >> 2), piece = (c0 >> 3) + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1);   // r0 is a multiple of 16
+      const T* at = s + (r0 + row) * D + ((piece ^ swz(row)) << 3) + (i & 1) * 4;
+      *(s16x4*)&x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+      *((s16x4*)&x + 1) = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * D));      // swz(row + 8) = swz(row)
+    }
+    return x;
+  }
+  // N rows from g on to LDS by direct loads; rows past `left` repeat the last one there is
+  template <int N, int THREADS> static __device__ __forceinline__ void load(T* s, const T* g, long long ld, int left) {
+    constexpr int kPieces = N * C / THREADS;
+    static_assert(N * C % THREADS == 0, "whole turns");
+    const unsigned dst = (unsigned)(size_t)(__attribute__((address_space(3))) void*)s + (unsigned)__builtin_amdgcn_readfirstlane((threadIdx.x >> 6) << 10);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int L = i * THREADS + threadIdx.x, row = L / C, r = row < left ? row : left - 1;
+      lds_load16(g, (unsigned)(((unsigned)r * (unsigned)ld + (unsigned)(((L % C) ^ swz(row)) * V)) * (unsigned)sizeof(T)), dst + i * (THREADS * 16));
+    }
+  }
+};
+
+// acc[db] (C rows = columns db * 32 .. of D, C column = p's column) += X^T p, X = the 32 LDS rows from r0
+template <typename T, int D>
+__device__ __forceinline__ void add_across(f32x16 (&acc)[D / 32], const T* s, int r0, const f32x16& p) {
+  using vec = typename Elem<T>::vec;
+  constexpr int kStep = sizeof(T) == 4 ? 8 : 16;
+#pragma unroll
+  for (int g = 0; g < 32 / kStep; ++g) {
+    vec b;
+#pragma unroll
+    for (int e = 0; e < kStep / 2; ++e) b[e] = (T)p[g * (kStep / 2) + e];
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) Elem<T>::mma(Rows<T, D, kCol>::across(s, r0 + g * kStep, db * 32), b, acc[db]);
+  }
+}
+
+// line[kMargin + R + e] = bias(e) / scale, |e| <= R + kMargin: the start value of a tile's sums, so that a tile near the diagonal costs a
+// look-up a score and no arithmetic.  Finite values stay within what the later product with scale log2(e) can hold: a row
+// of the type's lowest value has a softmax.
+constexpr int kMargin = 64;
+template <typename T>
+__device__ __forceinline__ void make_start_line(float* line, const AttnParams& p, int head, float c) {
+  const float most = 3e38f / fmaxf(c, 1.f);
+  for (int t = threadIdx.x; t <= 2 * (p.reach + kMargin); t += blockDim.x) {
+    const float b = (float)((const T*)p.table)[(long long)bucket_of(p.bk, t - p.reach - kMargin) * p.heads + head];
+    line[t] = __builtin_isinf(b) ? b : fminf(fmaxf(b / p.scale, -most), most);
+  }
+}
+
+// The block's place: contiguous runs of (head, slot) per XCD, so that the blocks that read one sequence's keys share an L2.
+__device__ __forceinline__ unsigned xcd_run(unsigned n) {
+  const unsigned x = blockIdx.x & 7, q = blockIdx.x >> 3;
+  return x * (n >> 3) + (x < (n & 7) ? x : (n & 7)) + q;
+}
+
+// C registers -> D / 32 column blocks of the wave's 32 rows, through LDS of the wave's own, as whole rows
+template <typename T, int D>
+__device__ __forceinline__ void store_turned(T* mine, T* dst, long long ld, const f32x16 (&acc)[D / 32], float f, int rows) {
+  using R = Rows<T, D, kRow>;
+  typedef T vec4 __attribute__((ext_vector_type(4)));
+  const int lane = threadIdx.x & 63, half = lane >> 5, l = lane & 31;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = db * 32 + 8 * g + 4 * half;
+      vec4 o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = (T)(acc[db][4 * g + e] * f);
+      *(vec4*)(mine + l * D + (((c / R::V) ^ R::swz(l)) * R::V) + (c & (R::V - 1))) = o;
+    }
+  asm volatile("" ::: "memory");       // a wave's LDS operations keep their order
+#pragma unroll
+  for (int i = 0; i < 32 * R::C / 64; ++i) {
+    const int L = i * 64 + lane, row = L / R::C, c = L % R::C;
+    const i32x4 v = *(const i32x4*)(mine + row * D + ((c ^ R::swz(row)) * R::V));
+    if (row < rows) *(i32x4*)(dst + row * ld + c * R::V) = v;
+  }
+  asm volatile("" ::: "memory");
+}
+
+// Block: one slot of NW * 32 queries of one head, 32 queries a wave, one per lane column; key tiles of 64, the next one under way
+// while one is multiplied.  Per score: one product-and-add, one exponential, half a maximum, one sum, half a conversion; the
+// running sums are rescaled only when a maximum has moved.
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams p, unsigned slots) {
+  constexpr int BQ = NW * 32, KT = 64, V = Elem<T>::kVec;
+  using KR = Rows<T, D, kRow>;
+  using VR = Rows<T, D, kCol>;
+  __shared__ __align__(1024) T buf[2][2][KT * D];          // [turn][k, v]
+  extern __shared__ float line[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l = lane & 31;
+  const unsigned at = xcd_run(slots * p.heads);
+  const int head = at / slots;
+  const Slot s = find_slot(p.offsets, p.n_seqs, p.total, BQ, at % slots);
+  if (s.b < 0) return;
+  const long long hd = (long long)p.heads * D;
+  if (s.b == p.n_seqs) {
+    const long long r0 = s.begin + (long long)s.tile * BQ, r1 = r0 + BQ < s.end ? r0 + BQ : s.end;
+    zero_rows((T*)p.out + (long long)head * D, hd, r0, r1, D);
+    return;
+  }
+  const int len = (int)(s.end - s.begin), tiles = (len + KT - 1) / KT;
+  const int i0 = s.tile * BQ + wave * 32;
+  const T* kb = (const T*)p.k + s.begin * p.ld_t + head * p.ld_h;
+  const T* vb = (const T*)p.v + s.begin * p.ld_t + head * p.ld_h;
+  auto issue = [&](int t) {
+    const int left = len - t * KT;
+    KR::template load<KT, NW * 64>(buf[t & 1][0], kb + (long long)t * KT * p.ld_t, p.ld_t, left);
+    VR::template load<KT, NW * 64>(buf[t & 1][1], vb + (long long)t * KT * p.ld_t, p.ld_t, left);
+  };
+  issue(0);
+  typename Elem<T>::vec fq[D / (2 * V)];
+  {
+    const int i = i0 + l < len ? i0 + l : len - 1;
+    const T* q = (const T*)p.q + (s.begin + i) * p.ld_t + head * p.ld_h + half * V;
+#pragma unroll
+    for (int x = 0; x < D / (2 * V); ++x) fq[x] = *(const typename Elem<T>::vec*)(q + x * 2 * V);
+  }
+  const float c = p.scale * kLog2e;
+  make_start_line<T>(line, p, head, c);
+  const float* mid = line + p.reach + kMargin + 4 * half - l;      // mid[e0 + row] = start value of row (+ 4 half), column l
+  float m = -INFINITY, sum = 0.f;
+  f32x16 acc[D / 32] = {};
+  for (int t = 0; t < tiles; ++t) {
+    wait_loads<0>();
+    __syncthreads();
+    if (t + 1 < tiles) issue(t + 1);
+    if (i0 >= len) continue;
+    const T* sk = buf[t & 1][0];
+    const T* sv = buf[t & 1][1];
+    const int j0 = t * KT;
+    f32x16 x[2];
+    float shift[2] = {0.f, 0.f};         // a far tile's bias, added behind the product
+    float top = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int e0 = j0 + u * 32 - i0;
+      if (e0 - 31 >= p.reach || e0 + 31 <= -p.reach) {
+        shift[u] = line[e0 > 0 ? 2 * (p.reach + kMargin) : 0] * c;
+        x[u] = f32x16{};
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[u][r] = mid[e0 + (r & 3) + 8 * (r >> 2)];
+      }
+#pragma unroll
+      for (int i = 0; i < D / (2 * V); ++i) Elem<T>::mma(KR::along(sk, u * 32, i), fq[i], x[u]);
+      if (j0 + u * 32 + 32 > len) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) if (j0 + u * 32 + (r & 3) + 8 * (r >> 2) + 4 * half >= len) x[u][r] = -INFINITY;
+      }
+      float high = x[u][0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) high = fmaxf(high, x[u][r]);
+      top = fmaxf(top, high * c + shift[u]);
+    }
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    if (__any(top > m)) {
+      const float m1 = fmaxf(m, top), fade = __builtin_amdgcn_exp2f(m - (m1 == -INFINITY ? 0.f : m1));
+      m = m1;
+      sum *= fade;
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db) acc[db] *= fade;
+    }
+    const float base = m == -INFINITY ? 0.f : m;       // a row of -inf alone: p = 0, not NaN
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const float off = shift[u] - base;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) { x[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][r], c, off)); sum += x[u][r]; }
+      add_across<T, D>(acc, sv, u * 32, x[u]);
+    }
+  }
+  __syncthreads();
+  if (i0 >= len) return;
+  sum += __shfl_xor(sum, 32, 64);
+  const bool any = sum > 0.f || sum != sum;
+  T* mine = &buf[0][0][0] + wave * (32 * D);
+  store_turned<T, D>(mine, (T*)p.out + (s.begin + i0) * hd + (long long)head * D, hd, acc, any ? 1.f / sum : 0.f, len - i0);
+  if (p.lse && lane < 32 && i0 + l < len) p.lse[(long long)head * p.total + s.begin + i0 + l] = any ? m + __log2f(sum) : INFINITY;
 }
 
 // ---- backward -------------------------------------------------------------------------------------------------------------
@@ -286,7 +497,7 @@ __device__ __forceinline__ float ds_lift(const AttnParams& p, int head, long lon
     const float po = __uint_as_float(p.peak[(long long)head * p.n_seqs + b]), pv = __uint_as_float(p.peak[((long long)p.heads + head) * p.n_seqs + b]);
     const float bound = 2.f * (float)p.d * po * pv;
     if (!(bound > 0.f) || bound > 1e30f || bound < 1e-30f) return 1.f;
-    return exp2f((float)(14 - ilogbf(bound)));
+    return ldexpf(1.f, 14 - ilogbf(bound));
   } else {
     return 1.f;
   }
@@ -350,7 +561,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnParams 
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int j = j0 + (r & 3) + 8 * (r >> 2) + 4 * half;
-      const float w = j < len ? exp2f(t[r] - lse) : 0.f;
+      const float w = j < len ? __builtin_amdgcn_exp2f(t[r] - lse) : 0.f;
       t[r] = w == 0.f ? 0.f : w * (dp[r] - delta);
     }
     if constexpr (DTABLE) {
@@ -443,7 +654,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_kernel(const AttnParams
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int row = (r & 3) + 8 * (r >> 2) + 4 * half;
-      t[r] = exp2f(t[r] - sl[row]);
+      t[r] = __builtin_amdgcn_exp2f(t[r] - sl[row]);
       ds[r] = t[r] == 0.f ? 0.f : t[r] * (dp[r] - sd[row]);
     }
     trans_times<T, DP>(av, sgt, t);

@@ -10,6 +10,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#pragma clang diagnostic ignored "-Winline-asm"   // m0 on a clobber list (it is reserved; nothing else in these kernels uses it)
 
 namespace vdbk {
 
@@ -45,6 +46,16 @@ template <> struct Elem<_Float16> {
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
+
+// ---- direct loads to LDS ------------------------------------------------------------------------------------------
+// 64 lanes x 16 bytes from sbase + voff to LDS lds_dst + 16 lane; waited for by hand (the compiler does not see the load).
+__device__ __forceinline__ void lds_load16(const void* sbase, unsigned voff, unsigned lds_dst) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "s"(lds_dst) : "memory", "m0");
+}
+template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory"); }
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 // ---- activations and their slopes, fp32 -----------------------------------------------------------------------
 // The normal distribution's integral Phi(z), and exp(-z^2 / 2).  fp32 operands: erff.  16-bit operands: Abramowitz and Stegun's

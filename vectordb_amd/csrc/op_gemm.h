@@ -1,7 +1,6 @@
 // op_gemm.h — C[i][j] = sum_c A(i, c) B(j, c) with the linear layer's epilogue, for every size, stride and alignment.
 #pragma once
 #include "op_common.h"
-#pragma clang diagnostic ignored "-Winline-asm"   // m0 on a clobber list (it is reserved; nothing else in these kernels uses it)
 
 namespace vdbk {
 
@@ -131,11 +130,6 @@ __global__ __launch_bounds__(256) void gemm_any_kernel(const GemmParams p) {
 //
 // Edges: rows past the end repeat the last (never stored); contracted values past the end are zeros written by the lane that
 // would have loaded them.
-__device__ __forceinline__ void lds_load16(const void* sbase, unsigned voff, unsigned lds_dst) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "s"(lds_dst) : "memory", "m0");
-}
-template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory"); }
-
 // 16x16 tiles: one 16-byte fragment contracts 32 (16-bit: one instruction) or 16 (fp32: four) values
 template <typename T> struct Frag16;
 template <> struct Frag16<float> {
@@ -150,9 +144,6 @@ template <> struct Frag16<_Float16> {
   static constexpr int kIns = 1;
   static __device__ __forceinline__ void mma(f16x8 a, f16x8 b, f32x4& c, int) { c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
-
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 template <typename T, bool ACROSS, int ROWS, int THREADS>
 struct TileOperand {
