@@ -42,11 +42,27 @@ hipError_t backward(const AttnParams& p, const AttnArgs& a) {
   const int64_t slots = n_slots(p.total, p.n_seqs, NW * 32);
   const unsigned grid = (unsigned)(slots * p.heads);
   const size_t line = (2 * p.reach + 1) * sizeof(float), hist = (size_t)NW * 2 * 2 * (p.reach + 64) * sizeof(float);
-  if (a.dtable) attention_dq_kernel<T, DP, NW, true><<<grid, NW * 64, line + hist, a.st>>>(p);
-  else attention_dq_kernel<T, DP, NW, false><<<grid, NW * 64, line, a.st>>>(p);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  attention_dkv_kernel<T, DP, NW><<<grid, NW * 64, line, a.st>>>(p);
+  hipError_t e;
+  // fp32 heads of 128 stay with the general kernels: two gradients and two operands of 128 words a row are more than the 512
+  // registers of a lane
+  constexpr bool kTiled = sizeof(T) * DP < 512;
+  bool done = false;
+  if constexpr (kTiled) {
+    if (p.vec && p.d == DP) {
+      const size_t start = (2 * (p.reach + kMargin) + 1) * sizeof(float);
+      if (a.dtable) attention_dq_kernel<T, DP, NW, true><<<grid, NW * 64, start + hist, a.st>>>(p, (unsigned)slots);
+      else attention_dq_kernel<T, DP, NW, false><<<grid, NW * 64, start, a.st>>>(p, (unsigned)slots);
+      if ((e = hipGetLastError()) != hipSuccess) return e;
+      attention_dkv_kernel<T, DP, NW><<<grid, NW * 64, start, a.st>>>(p, (unsigned)slots);
+      done = true;
+    }
+  }
+  if (!done) {
+    if (a.dtable) attention_dq_any_kernel<T, DP, NW, true><<<grid, NW * 64, line + hist, a.st>>>(p);
+    else attention_dq_any_kernel<T, DP, NW, false><<<grid, NW * 64, line, a.st>>>(p);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    attention_dkv_any_kernel<T, DP, NW><<<grid, NW * 64, line, a.st>>>(p);
+  }
   if ((e = hipGetLastError()) != hipSuccess || !a.dtable) return e;
   attention_dtable_kernel<T><<<(unsigned)(p.heads * p.n_buckets), 256, 0, a.st>>>(p.part, slots, p.heads, p.n_buckets, (T*)a.dtable);
   return hipGetLastError();

@@ -452,6 +452,25 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams 
   if (p.lse && lane < 32 && i0 + l < len) p.lse[(long long)head * p.total + s.begin + i0 + l] = any ? m + __log2f(sum) : INFINITY;
 }
 
+// part[t] = bucket t's sum of the waves' lines hist [2 waves][span] by distance and of what lies beyond R (far): one thread per bucket,
+// in order.
+__device__ __forceinline__ void fold_buckets(const AttnParams& p, const float* hist, const float (*far)[2], int waves, int span, float* part) {
+  for (int t = threadIdx.x; t < p.n_buckets; t += blockDim.x) {
+    const int low = t % p.bk.half, side = t / p.bk.half;
+    const int n0 = low <= p.bk.near ? low : p.bk.step[low - p.bk.near - 1];
+    const int n1 = low + 1 == p.bk.half ? span / 2 : low + 1 <= p.bk.near ? low + 1 : p.bk.step[low - p.bk.near];
+    float x = 0.f;
+    for (int w = 0; w < waves; ++w) {
+      if (low + 1 == p.bk.half) x += far[w][side];
+      for (int g = 0; g < 2; ++g) {
+        const float* h = hist + (w * 2 + g) * span + span / 2;
+        for (int n = side ? (n0 > 1 ? n0 : 1) : n0; n < n1; ++n) x += h[side ? n : -n];
+      }
+    }
+    part[t] = x;
+  }
+}
+
 // ---- backward -------------------------------------------------------------------------------------------------------------
 // delta[h][t] = sum_d dout out; fp16 also the largest |dout| and |v| of each sequence and head (bits of non-negative
 // floats order like integers, so the atomic maximum does not depend on the order of arrival).
@@ -509,7 +528,7 @@ __device__ __forceinline__ float ds_lift(const AttnParams& p, int head, long lon
 // at every step, and a wave's LDS operations keep their order, so nothing depends on timing.  Tiles beyond R go into two
 // registers.  One thread per bucket then adds up its distances, in order.
 template <typename T, int DP, int NW, bool DTABLE>
-__global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnParams p) {
+__global__ __launch_bounds__(NW * 64) void attention_dq_any_kernel(const AttnParams p) {
   constexpr int V = Elem<T>::kVec, BQ = NW * 32;
   __shared__ __align__(16) T sk[32 * (DP + V)];
   __shared__ __align__(16) T skt[DP * (32 + V)];
@@ -586,26 +605,13 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_kernel(const AttnParams 
     for (int k = 32; k; k >>= 1) { below += __shfl_xor(below, k, 64); above += __shfl_xor(above, k, 64); }
     if (lane == 0) { far[wave][0] = below; far[wave][1] = above; }
     __syncthreads();
-    for (int t = threadIdx.x; t < p.n_buckets; t += NW * 64) {
-      const int low = t % p.bk.half, side = t / p.bk.half;        // t < 2 half
-      const int n0 = low <= p.bk.near ? low : p.bk.step[low - p.bk.near - 1];
-      const int n1 = low + 1 == p.bk.half ? reach + 64 : low + 1 <= p.bk.near ? low + 1 : p.bk.step[low - p.bk.near];
-      float x = 0.f;
-      for (int w = 0; w < NW; ++w) {
-        if (low + 1 == p.bk.half) x += far[w][side];
-        for (int g = 0; g < 2; ++g) {
-          const float* h = hist + (w * 2 + g) * span + reach + 64;
-          for (int n = side ? (n0 > 1 ? n0 : 1) : n0; n < n1; ++n) x += h[side ? n : -n];
-        }
-      }
-      part[t] = x;
-    }
+    fold_buckets(p, hist, far, NW, span, part);
   }
 }
 
 // dk and dv: block = NW * 32 keys of one head, one key per lane column; query tiles of 32 through LDS.
 template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64) void attention_dkv_kernel(const AttnParams p) {
+__global__ __launch_bounds__(NW * 64) void attention_dkv_any_kernel(const AttnParams p) {
   constexpr int V = Elem<T>::kVec, BQ = NW * 32;
   __shared__ __align__(16) T sq[32 * (DP + V)];
   __shared__ __align__(16) T sqt[DP * (32 + V)];
@@ -664,6 +670,223 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_kernel(const AttnParams
   if (j >= len) return;
   store_cols<T, DP>((T*)p.dk + (s.begin + j) * p.gld_t + head * p.gld_h, ak, p.scale / lift, p.d, p.vec);
   store_cols<T, DP>((T*)p.dv + (s.begin + j) * p.gld_t + head * p.gld_h, av, 1.f, p.d, p.vec);
+}
+
+// ---- backward, whole 16-byte pieces and head widths of 32, 64 and 128 -------------------------------------------------------
+// dq and the block's bucket sums.  Each wave: 32 queries, one per lane column; key tiles of 64 through LDS.  k is read along its rows (scores) and across them (ds k): one copy in LDS, in the order of the transposed reads, serves
+// both - the reads along it meet two by two on a bank.
+template <typename T, int D, int NW, bool DTABLE>
+__global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel(const AttnParams p, unsigned slots) {
+  constexpr int BQ = NW * 32, KT = 64, V = Elem<T>::kVec;
+  using R = Rows<T, D, kCol>;
+  using RV = Rows<T, D, kRow>;
+  __shared__ __align__(1024) T buf[2][2][KT * D];          // [turn][k, v]
+  __shared__ float far[NW][2];
+  extern __shared__ float line[];                          // 2 (R + margin) + 1, then NW * 2 lines of 2 (R + margin)
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l = lane & 31;
+  const unsigned at = xcd_run(slots * p.heads);
+  const int head = at / slots;
+  const unsigned slot = at % slots;
+  const Slot s = find_slot(p.offsets, p.n_seqs, p.total, BQ, slot);
+  float* part = p.part + ((long long)slot * p.heads + head) * p.n_buckets;
+  if (s.b < 0 || s.b == p.n_seqs) {
+    if (s.b >= 0) {
+      const long long r0 = s.begin + (long long)s.tile * BQ, r1 = r0 + BQ < s.end ? r0 + BQ : s.end;
+      zero_rows((T*)p.dq + head * p.gld_h, p.gld_t, r0, r1, D);
+    }
+    if constexpr (DTABLE) for (int t = threadIdx.x; t < p.n_buckets; t += NW * 64) part[t] = 0.f;
+    return;
+  }
+  const int len = (int)(s.end - s.begin), tiles = (len + KT - 1) / KT;
+  const int i0 = s.tile * BQ + wave * 32;
+  const int reach = p.reach, span = 2 * (reach + kMargin);
+  const T* kb = (const T*)p.k + s.begin * p.ld_t + head * p.ld_h;
+  const T* vb = (const T*)p.v + s.begin * p.ld_t + head * p.ld_h;
+  auto issue = [&](int t) {
+    const int left = len - t * KT;
+    R::template load<KT, NW * 64>(buf[t & 1][0], kb + (long long)t * KT * p.ld_t, p.ld_t, left);
+    RV::template load<KT, NW * 64>(buf[t & 1][1], vb + (long long)t * KT * p.ld_t, p.ld_t, left);
+  };
+  issue(0);
+  const long long hd = (long long)p.heads * D;
+  using vec = typename Elem<T>::vec;
+  vec fq[D / (2 * V)], fg[D / (2 * V)];
+  const int i = i0 + l < len ? i0 + l : len - 1;
+  {
+    const T* q = (const T*)p.q + (s.begin + i) * p.ld_t + head * p.ld_h + half * V;
+    const T* g = (const T*)p.dout + (s.begin + i) * hd + (long long)head * D + half * V;
+#pragma unroll
+    for (int x = 0; x < D / (2 * V); ++x) { fq[x] = *(const vec*)(q + x * 2 * V); fg[x] = *(const vec*)(g + x * 2 * V); }
+  }
+  const long long row = (long long)head * p.total + s.begin + i;
+  const float lse = i0 + l < len ? p.lse[row] : INFINITY, delta = p.delta[row];
+  const float lift = ds_lift<T>(p, head, s.b);
+  const float c = p.scale * kLog2e;
+  float* hist = line + span + 1;
+  make_start_line<T>(line, p, head, c);
+  if constexpr (DTABLE) for (int t = threadIdx.x; t < NW * 2 * span; t += NW * 64) hist[t] = 0.f;
+  const float* mid = line + reach + kMargin + 4 * half - l;
+  float* mine = hist + (wave * 2 + half) * span + reach + kMargin + 4 * half - l;       // mine[e0 + row]
+  float below = 0.f, above = 0.f;
+  f32x16 acc[D / 32] = {};
+  for (int t = 0; t < tiles; ++t) {
+    wait_loads<0>();
+    __syncthreads();
+    if (t + 1 < tiles) issue(t + 1);
+    if (i0 >= len) continue;
+    const T* sk = buf[t & 1][0];
+    const T* sv = buf[t & 1][1];
+#pragma unroll
+    for (int u = 0; u < KT / 32; ++u) {
+      const int j0 = t * KT + u * 32, e0 = j0 - i0;
+      if (j0 >= len) break;
+      const bool is_far = e0 - 31 >= reach || e0 + 31 <= -reach;
+      f32x16 x, dp = {};
+      float shift = -lse;
+      if (is_far) {
+        shift += line[e0 > 0 ? span : 0] * c;
+        x = f32x16{};
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = mid[e0 + (r & 3) + 8 * (r >> 2)];
+      }
+#pragma unroll
+      for (int y = 0; y < D / (2 * V); ++y) Elem<T>::mma(R::along(sk, u * 32, y), fq[y], x);
+#pragma unroll
+      for (int y = 0; y < D / (2 * V); ++y) Elem<T>::mma(RV::along(sv, u * 32, y), fg[y], dp);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], c, shift));
+        x[r] = w == 0.f ? 0.f : w * (dp[r] - delta);       // a forbidden place may hold anything
+      }
+      if (j0 + 32 > len) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) if (j0 + (r & 3) + 8 * (r >> 2) + 4 * half >= len) x[r] = 0.f;
+      }
+      if constexpr (DTABLE) {
+        if (is_far) {
+          float y = 0.f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) y += x[r];
+          if (e0 > 0) above += y; else below += y;
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) __hip_atomic_fetch_add(mine + e0 + (r & 3) + 8 * (r >> 2), x[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+        }
+      }
+      if (lift != 1.f) x *= lift;
+      add_across<T, D>(acc, sk, u * 32, x);
+    }
+  }
+  __syncthreads();
+  if (i0 < len) store_turned<T, D>(&buf[0][0][0] + wave * (32 * D), (T*)p.dq + (s.begin + i0) * p.gld_t + head * p.gld_h, p.gld_t, acc, p.scale / lift, len - i0);
+  if constexpr (DTABLE) {
+    for (int k = 32; k; k >>= 1) { below += __shfl_xor(below, k, 64); above += __shfl_xor(above, k, 64); }
+    if (lane == 0) { far[wave][0] = below; far[wave][1] = above; }
+    __syncthreads();
+    fold_buckets(p, hist, far, NW, span, part);
+  }
+}
+
+// dk and dv: each wave 32 keys, one per lane column; query tiles of 64 through LDS, q and dout once, in the order of the
+// transposed reads.
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kernel(const AttnParams p, unsigned slots) {
+  constexpr int BQ = NW * 32, QT = 64, V = Elem<T>::kVec;
+  using R = Rows<T, D, kCol>;
+  using vec = typename Elem<T>::vec;
+  __shared__ __align__(1024) T buf[2][2][QT * D];       // [turn][q, dout]
+  __shared__ __align__(16) float stat[2][2][QT];             // [turn][lse, delta]
+  extern __shared__ float line[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l = lane & 31;
+  const unsigned at = xcd_run(slots * p.heads);
+  const int head = at / slots;
+  const Slot s = find_slot(p.offsets, p.n_seqs, p.total, BQ, at % slots);
+  if (s.b < 0) return;
+  if (s.b == p.n_seqs) {
+    const long long r0 = s.begin + (long long)s.tile * BQ, r1 = r0 + BQ < s.end ? r0 + BQ : s.end;
+    zero_rows((T*)p.dk + head * p.gld_h, p.gld_t, r0, r1, D);
+    zero_rows((T*)p.dv + head * p.gld_h, p.gld_t, r0, r1, D);
+    return;
+  }
+  const int len = (int)(s.end - s.begin), tiles = (len + QT - 1) / QT;
+  const int j0 = s.tile * BQ + wave * 32;
+  const long long hd = (long long)p.heads * D;
+  const T* qb = (const T*)p.q + s.begin * p.ld_t + head * p.ld_h;
+  const T* gb = (const T*)p.dout + s.begin * hd + (long long)head * D;
+  const float* lse = p.lse + (long long)head * p.total + s.begin;
+  const float* delta = p.delta + (long long)head * p.total + s.begin;
+  float next_lse = 0.f, next_delta = 0.f;    // thread x < QT: of query x of the tile under way
+  auto issue = [&](int t) {
+    const int left = len - t * QT;
+    R::template load<QT, NW * 64>(buf[t & 1][0], qb + (long long)t * QT * p.ld_t, p.ld_t, left);
+    R::template load<QT, NW * 64>(buf[t & 1][1], gb + (long long)t * QT * hd, hd, left);
+    if (threadIdx.x < QT) {
+      const bool there = (int)threadIdx.x < left;
+      next_lse = there ? lse[t * QT + threadIdx.x] : INFINITY;
+      next_delta = there ? delta[t * QT + threadIdx.x] : 0.f;
+    }
+  };
+  issue(0);
+  vec fk[D / (2 * V)], fv[D / (2 * V)];
+  {
+    const long long j = s.begin + (j0 + l < len ? j0 + l : len - 1);
+    const T* k = (const T*)p.k + j * p.ld_t + head * p.ld_h + half * V;
+    const T* v = (const T*)p.v + j * p.ld_t + head * p.ld_h + half * V;
+#pragma unroll
+    for (int x = 0; x < D / (2 * V); ++x) { fk[x] = *(const vec*)(k + x * 2 * V); fv[x] = *(const vec*)(v + x * 2 * V); }
+  }
+  const float lift = ds_lift<T>(p, head, s.b);
+  const float c = p.scale * kLog2e;
+  make_start_line<T>(line, p, head, c);
+  const float* mid = line + p.reach + kMargin - 4 * half + l;        // mid[e0 - row]: column l is the key, the rows are queries
+  f32x16 ak[D / 32] = {}, av[D / 32] = {};
+  for (int t = 0; t < tiles; ++t) {
+    if (threadIdx.x < QT) { stat[t & 1][0][threadIdx.x] = next_lse; stat[t & 1][1][threadIdx.x] = next_delta; }
+    wait_loads<0>();
+    __syncthreads();
+    if (t + 1 < tiles) issue(t + 1);
+    if (j0 >= len) continue;
+    const T* sq = buf[t & 1][0];
+    const T* sg = buf[t & 1][1];
+#pragma unroll
+    for (int u = 0; u < QT / 32; ++u) {
+      if (t * QT + u * 32 >= len) break;
+      const int e0 = j0 - t * QT - u * 32;
+      f32x16 x, dp = {};
+      float shift = 0.f;
+      if (e0 - 31 >= p.reach || e0 + 31 <= -p.reach) {
+        shift = line[e0 > 0 ? 2 * (p.reach + kMargin) : 0] * c;
+        x = f32x16{};
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = mid[e0 - (r & 3) - 8 * (r >> 2)];
+      }
+#pragma unroll
+      for (int y = 0; y < D / (2 * V); ++y) Elem<T>::mma(R::along(sq, u * 32, y), fk[y], x);
+#pragma unroll
+      for (int y = 0; y < D / (2 * V); ++y) Elem<T>::mma(R::along(sg, u * 32, y), fv[y], dp);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 ls = *(const f32x4*)&stat[t & 1][0][u * 32 + 8 * g + 4 * half], dl = *(const f32x4*)&stat[t & 1][1][u * 32 + 8 * g + 4 * half];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * g + e;
+          x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], c, shift - ls[e]));
+          dp[r] = x[r] == 0.f ? 0.f : x[r] * (dp[r] - dl[e]);       // a forbidden place may hold anything
+        }
+      }
+      add_across<T, D>(av, sg, u * 32, x);
+      if (lift != 1.f) dp *= lift;
+      add_across<T, D>(ak, sq, u * 32, dp);
+    }
+  }
+  __syncthreads();
+  if (j0 >= len) return;
+  // 32 rows at a time through the wave's part of LDS
+  T* mine = &buf[0][0][0] + wave * (32 * D);
+  store_turned<T, D>(mine, (T*)p.dk + (s.begin + j0) * p.gld_t + head * p.gld_h, p.gld_t, ak, p.scale / lift, len - j0);
+  store_turned<T, D>(mine, (T*)p.dv + (s.begin + j0) * p.gld_t + head * p.gld_h, p.gld_t, av, 1.f, len - j0);
 }
 
 // dtable[t][h] = the slots' parts in order, in 64 bits: block = one head and bucket
