@@ -37,18 +37,19 @@ hipError_t forward(const AttnParams& p, hipStream_t st) {
   return hipGetLastError();
 }
 
+// Which backward kernels serve.  fp32 heads of 128 stay with the general ones: two gradients and two operands of 128 words a row
+// are more than the 512 registers of a lane.
+template <typename T> bool tiled(const AttnParams& p) { return p.vec && (p.d == 32 || p.d == 64 || (p.d == 128 && sizeof(T) == 2)); }
+
 template <typename T, int DP, int NW>
 hipError_t backward(const AttnParams& p, const AttnArgs& a) {
   const int64_t slots = n_slots(p.total, p.n_seqs, NW * 32);
   const unsigned grid = (unsigned)(slots * p.heads);
   const size_t line = (2 * p.reach + 1) * sizeof(float), hist = (size_t)NW * 2 * 2 * (p.reach + 64) * sizeof(float);
   hipError_t e;
-  // fp32 heads of 128 stay with the general kernels: two gradients and two operands of 128 words a row are more than the 512
-  // registers of a lane
-  constexpr bool kTiled = sizeof(T) * DP < 512;
   bool done = false;
-  if constexpr (kTiled) {
-    if (p.vec && p.d == DP) {
+  if constexpr (sizeof(T) * DP < 512) {
+    if (tiled<T>(p)) {
       const size_t start = (2 * (p.reach + kMargin) + 1) * sizeof(float);
       if (a.dtable) attention_dq_kernel<T, DP, NW, true><<<grid, NW * 64, start + hist, a.st>>>(p, (unsigned)slots);
       else attention_dq_kernel<T, DP, NW, false><<<grid, NW * 64, start, a.st>>>(p, (unsigned)slots);
@@ -87,7 +88,7 @@ hipError_t run_t(const AttnArgs& a, bool back) {
       const long long n = 2ll * p.heads * p.n_seqs;
       if (n) fill_zero_kernel<<<(unsigned)std::min<long long>((n + 255) / 256, 1024), 256, 0, a.st>>>((unsigned*)a.gscale, n);
       attention_delta_kernel<T, true><<<grid, 256, 0, a.st>>>(p, (unsigned*)a.gscale);
-    } else {
+    } else if (!tiled<T>(p)) {
       attention_delta_kernel<T, false><<<grid, 256, 0, a.st>>>(p, nullptr);
     }
     hipError_t e = hipGetLastError();

@@ -452,27 +452,33 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams 
   if (p.lse && lane < 32 && i0 + l < len) p.lse[(long long)head * p.total + s.begin + i0 + l] = any ? m + __log2f(sum) : INFINITY;
 }
 
-// part[t] = bucket t's sum of the waves' lines hist [2 waves][span] by distance and of what lies beyond R (far): one thread per bucket,
-// in order.
-__device__ __forceinline__ void fold_buckets(const AttnParams& p, const float* hist, const float (*far)[2], int waves, int span, float* part) {
-  for (int t = threadIdx.x; t < p.n_buckets; t += blockDim.x) {
-    const int low = t % p.bk.half, side = t / p.bk.half;
-    const int n0 = low <= p.bk.near ? low : p.bk.step[low - p.bk.near - 1];
-    const int n1 = low + 1 == p.bk.half ? span / 2 : low + 1 <= p.bk.near ? low + 1 : p.bk.step[low - p.bk.near];
+// part[t] = bucket t's sum of the lines hist [lines][span] by distance and of what lies beyond R (far): the lines joined in order,
+// then eight lanes per bucket.
+__device__ __forceinline__ void fold_buckets(const AttnParams& p, float* hist, const float (*far)[2], int lines, int span, float* part) {
+  __syncthreads();
+  for (int t = threadIdx.x; t < span; t += blockDim.x) {
+    float x = hist[t];
+    for (int w = 1; w < lines; ++w) x += hist[w * span + t];
+    hist[t] = x;
+  }
+  __syncthreads();
+  const int sub = threadIdx.x & 7;
+  for (int t = threadIdx.x >> 3; t < ((p.n_buckets + 7) & ~7); t += blockDim.x >> 3) {
     float x = 0.f;
-    for (int w = 0; w < waves; ++w) {
-      if (low + 1 == p.bk.half) x += far[w][side];
-      for (int g = 0; g < 2; ++g) {
-        const float* h = hist + (w * 2 + g) * span + span / 2;
-        for (int n = side ? (n0 > 1 ? n0 : 1) : n0; n < n1; ++n) x += h[side ? n : -n];
-      }
+    if (t < p.n_buckets) {
+      const int low = t % p.bk.half, side = t / p.bk.half;
+      const int n0 = low <= p.bk.near ? low : p.bk.step[low - p.bk.near - 1];
+      const int n1 = low + 1 == p.bk.half ? span / 2 : low + 1 <= p.bk.near ? low + 1 : p.bk.step[low - p.bk.near];
+      for (int n = (side && n0 == 0 ? 1 : n0) + sub; n < n1; n += 8) x += hist[span / 2 + (side ? n : -n)];
+      if (sub == 0 && low + 1 == p.bk.half) for (int w = 0; w < lines / 2; ++w) x += far[w][side];
     }
-    part[t] = x;
+    for (int k = 1; k < 8; k <<= 1) x += __shfl_xor(x, k, 64);
+    if (sub == 0 && t < p.n_buckets) part[t] = x;
   }
 }
 
 // ---- backward -------------------------------------------------------------------------------------------------------------
-// delta[h][t] = sum_d dout out; fp16 also the largest |dout| and |v| of each sequence and head (bits of non-negative
+// delta[h][t] = sum_d dout out (the general kernels'; attention_dq_kernel has its own); fp16 also the largest |dout| and |v| of each sequence and head (bits of non-negative
 // floats order like integers, so the atomic maximum does not depend on the order of arrival).
 template <typename T, bool PEAK>
 __global__ __launch_bounds__(256) void attention_delta_kernel(const AttnParams p, unsigned* peak) {
@@ -604,8 +610,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_any_kernel(const AttnPar
   if constexpr (DTABLE) {
     for (int k = 32; k; k >>= 1) { below += __shfl_xor(below, k, 64); above += __shfl_xor(above, k, 64); }
     if (lane == 0) { far[wave][0] = below; far[wave][1] = above; }
-    __syncthreads();
-    fold_buckets(p, hist, far, NW, span, part);
+    fold_buckets(p, hist, far, NW * 2, span, part);
   }
 }
 
@@ -673,6 +678,26 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_any_kernel(const AttnPa
 }
 
 // ---- backward, whole 16-byte pieces and head widths of 32, 64 and 128 -------------------------------------------------------
+// A 32x32 tile's sums by distance, keys in the registers: every register's 32 lanes of a half are turned by their row number, which
+// brings equal distances to one lane; what wraps round goes to a second sum.  Sixteen lane moves and two additions to the
+// half's line in LDS; adding each score to the line by LDS atomics instead cost 250 us of a 428 us pass (64 texts of 16 to 384
+// tokens, 12 heads).
+__device__ __forceinline__ void add_diagonals(float* mine, int e0, const f32x16& x) {
+  const int lane = threadIdx.x & 63, l = lane & 31;
+  float a = 0.f, b = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int row = (r & 3) + 8 * (r >> 2);
+    const float v = __int_as_float(__builtin_amdgcn_ds_bpermute(((lane & 32) | ((l + row) & 31)) << 2, __float_as_int(x[r])));
+    const bool in = l + row < 32;          // the value's column is l + row: distance -l, or beyond the edge 32 - l
+    a += in ? v : 0.f;
+    b += in ? 0.f : v;
+  }
+  // 32 distances each, no two lanes of a half alike; a wave's LDS operations keep their order
+  __hip_atomic_fetch_add(mine + e0 - l, a, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+  __hip_atomic_fetch_add(mine + e0 - l + 32, b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+}
+
 // dq and the block's bucket sums.  Each wave: 32 queries, one per lane column; key tiles of 64 through LDS.  k is read along its rows (scores) and across them (ds k): one copy in LDS, in the order of the transposed reads, serves
 // both - the reads along it meet two by two on a bank.
 template <typename T, int D, int NW, bool DTABLE>
@@ -719,14 +744,26 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
     for (int x = 0; x < D / (2 * V); ++x) { fq[x] = *(const vec*)(q + x * 2 * V); fg[x] = *(const vec*)(g + x * 2 * V); }
   }
   const long long row = (long long)head * p.total + s.begin + i;
-  const float lse = i0 + l < len ? p.lse[row] : INFINITY, delta = p.delta[row];
+  const float lse = i0 + l < len ? p.lse[row] : INFINITY;
+  float delta = 0.f;                 // dout . out, for this kernel and, through memory, for dk
+  {
+    const T* o = (const T*)p.out + (s.begin + i) * hd + (long long)head * D + half * V;
+#pragma unroll
+    for (int x = 0; x < D / (2 * V); ++x) {
+      const vec fo = *(const vec*)(o + x * 2 * V);
+#pragma unroll
+      for (int e = 0; e < V; ++e) delta += (float)fo[e] * (float)fg[x][e];
+    }
+    delta += __shfl_xor(delta, 32, 64);
+    if (lane < 32 && i0 + l < len) p.delta[row] = delta;
+  }
   const float lift = ds_lift<T>(p, head, s.b);
   const float c = p.scale * kLog2e;
   float* hist = line + span + 1;
   make_start_line<T>(line, p, head, c);
   if constexpr (DTABLE) for (int t = threadIdx.x; t < NW * 2 * span; t += NW * 64) hist[t] = 0.f;
   const float* mid = line + reach + kMargin + 4 * half - l;
-  float* mine = hist + (wave * 2 + half) * span + reach + kMargin + 4 * half - l;       // mine[e0 + row]
+  float* mine = hist + (wave * 2 + half) * span + reach + kMargin + 4 * half;       // mine[e0 + row - column]
   float below = 0.f, above = 0.f;
   f32x16 acc[D / 32] = {};
   for (int t = 0; t < tiles; ++t) {
@@ -770,8 +807,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
           for (int r = 0; r < 16; ++r) y += x[r];
           if (e0 > 0) above += y; else below += y;
         } else {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) __hip_atomic_fetch_add(mine + e0 + (r & 3) + 8 * (r >> 2), x[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+          add_diagonals(mine, e0, x);
         }
       }
       if (lift != 1.f) x *= lift;
@@ -783,8 +819,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
   if constexpr (DTABLE) {
     for (int k = 32; k; k >>= 1) { below += __shfl_xor(below, k, 64); above += __shfl_xor(above, k, 64); }
     if (lane == 0) { far[wave][0] = below; far[wave][1] = above; }
-    __syncthreads();
-    fold_buckets(p, hist, far, NW, span, part);
+    fold_buckets(p, hist, far, NW * 2, span, part);
   }
 }
 
