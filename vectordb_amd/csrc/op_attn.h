@@ -33,7 +33,10 @@ __device__ __forceinline__ int bucket_of(const Buckets& bk, int e) {
   int b = n;
   if (n >= bk.near) {
     b = bk.near;
-    for (int i = 0; i < bk.n_steps; ++i) b += n >= bk.step[i];
+    for (int i = 0; i < bk.n_steps; i += 8) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) b += n >= bk.step[i + u];     // behind the last: never
+    }
   }
   return b + (e > 0 ? bk.half : 0);
 }
@@ -312,11 +315,14 @@ __device__ __forceinline__ void add_across(f32x16 (&acc)[D / 32], const T* s, in
 constexpr int kMargin = 64;
 template <typename T>
 __device__ __forceinline__ void make_start_line(float* line, const AttnParams& p, int head, float c) {
+  __shared__ float tab[128];
   const float most = 3e38f / fmaxf(c, 1.f);
-  for (int t = threadIdx.x; t <= 2 * (p.reach + kMargin); t += blockDim.x) {
-    const float b = (float)((const T*)p.table)[(long long)bucket_of(p.bk, t - p.reach - kMargin) * p.heads + head];
-    line[t] = __builtin_isinf(b) ? b : fminf(fmaxf(b / p.scale, -most), most);
+  for (int t = threadIdx.x; t < p.n_buckets; t += blockDim.x) {
+    const float b = (float)((const T*)p.table)[(long long)t * p.heads + head];
+    tab[t] = __builtin_isinf(b) ? b : fminf(fmaxf(b / p.scale, -most), most);
   }
+  __syncthreads();
+  for (int t = threadIdx.x; t <= 2 * (p.reach + kMargin); t += blockDim.x) line[t] = tab[bucket_of(p.bk, t - p.reach - kMargin)];
 }
 
 // The block's place: contiguous runs of (head, slot) per XCD, so that the blocks that read one sequence's keys share an L2.

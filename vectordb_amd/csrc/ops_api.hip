@@ -78,6 +78,7 @@ Buckets make_buckets(int n_buckets, int max_distance) {
     }
     b.step[i - 1] = n;
   }
+  for (int i = b.n_steps; i < kMaxSteps; ++i) b.step[i] = 0x7fffffff;
   return b;
 }
 
