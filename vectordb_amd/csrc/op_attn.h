@@ -325,10 +325,37 @@ __device__ __forceinline__ void make_start_line(float* line, const AttnParams& p
   for (int t = threadIdx.x; t <= 2 * (p.reach + kMargin); t += blockDim.x) line[t] = tab[bucket_of(p.bk, t - p.reach - kMargin)];
 }
 
+// Waits for what the compiler has loaded into x, here: left to itself it waits where x is used first, inside the loop over tiles, and
+// that wait counts the direct loads under way there, which it does not know of.
+template <typename X> __device__ __forceinline__ void settle(X& x) { asm volatile("" : "+v"(x)); }
+
 // The block's place: contiguous runs of (head, slot) per XCD, so that the blocks that read one sequence's keys share an L2.
 __device__ __forceinline__ unsigned xcd_run(unsigned n) {
   const unsigned x = blockIdx.x & 7, q = blockIdx.x >> 3;
   return x * (n >> 3) + (x < (n & 7) ? x : (n & 7)) + q;
+}
+
+// A 32x32 tile of scores: the LDS rows from r0 against the lane's row f.  Near the diagonal the sums start from the line (start[row]);
+// a far tile's start from nothing, without sixteen moves, and its one bias is returned for the caller to add behind the product.
+template <typename T, int D, typename ROWS, int SIGN>
+__device__ __forceinline__ float scores(f32x16& x, const T* s, int r0, const typename Elem<T>::vec (&f)[D / (2 * Elem<T>::kVec)], int e0, const AttnParams& p,
+                                        const float* line, const float* start) {
+  constexpr int N = D / (2 * Elem<T>::kVec);
+  float shift = 0.f;
+  const bool is_far = e0 - 31 >= p.reach || e0 + 31 <= -p.reach;
+  if (__builtin_amdgcn_readfirstlane(is_far)) {
+    shift = line[e0 > 0 ? 2 * (p.reach + kMargin) : 0];
+    f32x16 none = {};
+    Elem<T>::mma(ROWS::along(s, r0, 0), f[0], none);
+    x = none;
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = start[SIGN * ((r & 3) + 8 * (r >> 2))];
+    Elem<T>::mma(ROWS::along(s, r0, 0), f[0], x);
+  }
+#pragma unroll
+  for (int i = 1; i < N; ++i) Elem<T>::mma(ROWS::along(s, r0, i), f[i], x);
+  return shift;
 }
 
 // C registers -> D / 32 column blocks of the wave's 32 rows, through LDS of the wave's own, as whole rows
@@ -355,6 +382,14 @@ __device__ __forceinline__ void store_turned(T* mine, T* dst, long long ld, cons
     if (row < rows) *(i32x4*)(dst + row * ld + c * R::V) = v;
   }
   asm volatile("" ::: "memory");
+}
+
+// sum += a + b: of the values as the product with v takes them, two by one instruction where there is one
+template <typename T> __device__ __forceinline__ void add_pair(float& sum, float a, float b) {
+  typedef T pair __attribute__((ext_vector_type(2)));
+  if constexpr (__is_same(T, __bf16)) sum = __builtin_amdgcn_fdot2_f32_bf16(pair{(T)a, (T)b}, pair{(T)1.f, (T)1.f}, sum, false);
+  else if constexpr (__is_same(T, _Float16)) sum = __builtin_amdgcn_fdot2(pair{(T)a, (T)b}, pair{(T)1.f, (T)1.f}, sum, false);
+  else sum += a + b;
 }
 
 // Block: one slot of NW * 32 queries of one head, 32 queries a wave, one per lane column; key tiles of 64, the next one under way
@@ -398,6 +433,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams 
   const float c = p.scale * kLog2e;
   make_start_line<T>(line, p, head, c);
   const float* mid = line + p.reach + kMargin + 4 * half - l;      // mid[e0 + row] = start value of row (+ 4 half), column l
+#pragma unroll
+  for (int x = 0; x < D / (2 * V); ++x) settle(fq[x]);
   float m = -INFINITY, sum = 0.f;
   f32x16 acc[D / 32] = {};
   for (int t = 0; t < tiles; ++t) {
@@ -414,15 +451,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams 
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int e0 = j0 + u * 32 - i0;
-      if (e0 - 31 >= p.reach || e0 + 31 <= -p.reach) {
-        shift[u] = line[e0 > 0 ? 2 * (p.reach + kMargin) : 0] * c;
-        x[u] = f32x16{};
-      } else {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) x[u][r] = mid[e0 + (r & 3) + 8 * (r >> 2)];
-      }
-#pragma unroll
-      for (int i = 0; i < D / (2 * V); ++i) Elem<T>::mma(KR::along(sk, u * 32, i), fq[i], x[u]);
+      shift[u] = c * scores<T, D, KR, 1>(x[u], sk, u * 32, fq, e0, p, line, mid + e0);
       if (j0 + u * 32 + 32 > len) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) if (j0 + u * 32 + (r & 3) + 8 * (r >> 2) + 4 * half >= len) x[u][r] = -INFINITY;
@@ -445,7 +474,9 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams 
     for (int u = 0; u < 2; ++u) {
       const float off = shift[u] - base;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) { x[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][r], c, off)); sum += x[u][r]; }
+      for (int r = 0; r < 16; ++r) x[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][r], c, off));
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) add_pair<T>(sum, x[u][r], x[u][r + 1]);
       add_across<T, D>(acc, sv, u * 32, x[u]);
     }
   }
@@ -528,7 +559,7 @@ __device__ __forceinline__ float ds_lift(const AttnParams& p, int head, long lon
     const float po = __uint_as_float(p.peak[(long long)head * p.n_seqs + b]), pv = __uint_as_float(p.peak[((long long)p.heads + head) * p.n_seqs + b]);
     const float bound = 2.f * (float)p.d * po * pv;
     if (!(bound > 0.f) || bound > 1e30f || bound < 1e-30f) return 1.f;
-    return ldexpf(1.f, 14 - ilogbf(bound));
+    return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(ldexpf(1.f, 14 - ilogbf(bound)))));     // one value a block; waited for here
   } else {
     return 1.f;
   }
@@ -770,6 +801,11 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
   if constexpr (DTABLE) for (int t = threadIdx.x; t < NW * 2 * span; t += NW * 64) hist[t] = 0.f;
   const float* mid = line + reach + kMargin + 4 * half - l;
   float* mine = hist + (wave * 2 + half) * span + reach + kMargin + 4 * half;       // mine[e0 + row - column]
+#pragma unroll
+  for (int x = 0; x < D / (2 * V); ++x) { settle(fq[x]); settle(fg[x]); }
+  float from = -lse, less = delta;
+  settle(from);
+  settle(less);
   float below = 0.f, above = 0.f;
   f32x16 acc[D / 32] = {};
   for (int t = 0; t < tiles; ++t) {
@@ -785,22 +821,13 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
       if (j0 >= len) break;
       const bool is_far = e0 - 31 >= reach || e0 + 31 <= -reach;
       f32x16 x, dp = {};
-      float shift = -lse;
-      if (is_far) {
-        shift += line[e0 > 0 ? span : 0] * c;
-        x = f32x16{};
-      } else {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] = mid[e0 + (r & 3) + 8 * (r >> 2)];
-      }
-#pragma unroll
-      for (int y = 0; y < D / (2 * V); ++y) Elem<T>::mma(R::along(sk, u * 32, y), fq[y], x);
+      const float shift = from + c * scores<T, D, R, 1>(x, sk, u * 32, fq, e0, p, line, mid + e0);
 #pragma unroll
       for (int y = 0; y < D / (2 * V); ++y) Elem<T>::mma(RV::along(sv, u * 32, y), fg[y], dp);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], c, shift));
-        x[r] = w == 0.f ? 0.f : w * (dp[r] - delta);       // a forbidden place may hold anything
+        x[r] = w == 0.f ? 0.f : w * (dp[r] - less);       // a forbidden place may hold anything
       }
       if (j0 + 32 > len) {
 #pragma unroll
@@ -881,6 +908,8 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
   const float c = p.scale * kLog2e;
   make_start_line<T>(line, p, head, c);
   const float* mid = line + p.reach + kMargin - 4 * half + l;        // mid[e0 - row]: column l is the key, the rows are queries
+#pragma unroll
+  for (int x = 0; x < D / (2 * V); ++x) { settle(fk[x]); settle(fv[x]); }
   f32x16 ak[D / 32] = {}, av[D / 32] = {};
   for (int t = 0; t < tiles; ++t) {
     if (threadIdx.x < QT) { stat[t & 1][0][threadIdx.x] = next_lse; stat[t & 1][1][threadIdx.x] = next_delta; }
@@ -895,16 +924,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
       if (t * QT + u * 32 >= len) break;
       const int e0 = j0 - t * QT - u * 32;
       f32x16 x, dp = {};
-      float shift = 0.f;
-      if (e0 - 31 >= p.reach || e0 + 31 <= -p.reach) {
-        shift = line[e0 > 0 ? 2 * (p.reach + kMargin) : 0] * c;
-        x = f32x16{};
-      } else {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] = mid[e0 - (r & 3) - 8 * (r >> 2)];
-      }
-#pragma unroll
-      for (int y = 0; y < D / (2 * V); ++y) Elem<T>::mma(R::along(sq, u * 32, y), fk[y], x);
+      const float shift = c * scores<T, D, R, -1>(x, sq, u * 32, fk, e0, p, line, mid + e0);
 #pragma unroll
       for (int y = 0; y < D / (2 * V); ++y) Elem<T>::mma(R::along(sg, u * 32, y), fv[y], dp);
 #pragma unroll
