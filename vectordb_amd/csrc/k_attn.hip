@@ -28,11 +28,18 @@ AttnParams params(const AttnArgs& a, int elem) {
   return p;
 }
 
+// A prime that divides neither length that an XCD's run of n blocks can have
+unsigned hop_of(unsigned n) {
+  for (unsigned h : {61u, 67u, 71u, 73u, 79u, 83u, 89u, 97u, 101u, 103u, 107u, 109u, 113u, 127u, 131u})
+    if ((n >> 3) % h && ((n >> 3) + 1) % h) return h;
+  return 1;
+}
+
 template <typename T, int DP, int NW>
 hipError_t forward(const AttnParams& p, hipStream_t st) {
   const unsigned slots = (unsigned)n_slots(p.total, p.n_seqs, NW * 32), grid = slots * p.heads;
   if (p.vec && p.d == DP) {
-    attention_kernel<T, DP, NW><<<grid, NW * 64, (2 * (p.reach + kMargin) + 1) * sizeof(float), st>>>(p, slots);
+    attention_kernel<T, DP, NW><<<grid, NW * 64, (2 * (p.reach + kMargin) + 1) * sizeof(float), st>>>(p, slots, hop_of(grid));
     return hipGetLastError();
   }
   attention_any_kernel<T, DP, NW><<<grid, NW * 64, (2 * p.reach + 1) * sizeof(float), st>>>(p);
@@ -53,10 +60,10 @@ hipError_t backward(const AttnParams& p, const AttnArgs& a) {
   if constexpr (sizeof(T) * DP < 512) {
     if (tiled<T>(p)) {
       const size_t start = (2 * (p.reach + kMargin) + 1) * sizeof(float);
-      if (a.dtable) attention_dq_kernel<T, DP, NW, true><<<grid, NW * 64, start + hist, a.st>>>(p, (unsigned)slots);
-      else attention_dq_kernel<T, DP, NW, false><<<grid, NW * 64, start, a.st>>>(p, (unsigned)slots);
+      if (a.dtable) attention_dq_kernel<T, DP, NW, true><<<grid, NW * 64, start + hist, a.st>>>(p, (unsigned)slots, hop_of(grid));
+      else attention_dq_kernel<T, DP, NW, false><<<grid, NW * 64, start, a.st>>>(p, (unsigned)slots, hop_of(grid));
       if ((e = hipGetLastError()) != hipSuccess) return e;
-      attention_dkv_kernel<T, DP, NW><<<grid, NW * 64, start, a.st>>>(p, (unsigned)slots);
+      attention_dkv_kernel<T, DP, NW><<<grid, NW * 64, start, a.st>>>(p, (unsigned)slots, hop_of(grid));
       done = true;
     }
   }

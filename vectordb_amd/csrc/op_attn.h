@@ -329,10 +329,13 @@ __device__ __forceinline__ void make_start_line(float* line, const AttnParams& p
 // that wait counts the direct loads under way there, which it does not know of.
 template <typename X> __device__ __forceinline__ void settle(X& x) { asm volatile("" : "+v"(x)); }
 
-// The block's place: contiguous runs of (head, slot) per XCD, so that the blocks that read one sequence's keys share an L2.
-__device__ __forceinline__ unsigned xcd_run(unsigned n) {
-  const unsigned x = blockIdx.x & 7, q = blockIdx.x >> 3;
-  return x * (n >> 3) + (x < (n & 7) ? x : (n & 7)) + q;
+// The block's place: contiguous runs of (head, slot) per XCD, so that the blocks that read one sequence's keys share an L2; inside
+// its run an XCD takes the places `hop` apart (a prime that divides no run's length).  Blocks go to compute units in turn, and in
+// order the empty slots (one in four where every text has 384 tokens) would all fall to the same units: 16 x 384 tokens, 12 heads,
+// fp32, left a quarter of the chip idle.
+__device__ __forceinline__ unsigned xcd_run(unsigned n, unsigned hop) {
+  const unsigned x = blockIdx.x & 7, q = blockIdx.x >> 3, run = (n >> 3) + (x < (n & 7));
+  return x * (n >> 3) + (x < (n & 7) ? x : (n & 7)) + (unsigned)((unsigned long long)q * hop % run);
 }
 
 // A 32x32 tile of scores: the LDS rows from r0 against the lane's row f.  Near the diagonal the sums start from the line (start[row]);
@@ -392,18 +395,19 @@ template <typename T> __device__ __forceinline__ void add_pair(float& sum, float
   else sum += a + b;
 }
 
-// Block: one slot of NW * 32 queries of one head, 32 queries a wave, one per lane column; key tiles of 64, the next one under way
+// Block: one slot of NW * 32 queries of one head, 32 queries a wave, one per lane column; key tiles of 64 (fp32: 32, which lets
+// more blocks share a compute unit: 576 blocks of 16 x 384 tokens, 12 heads, would take two turns of 512), the next one under way
 // while one is multiplied.  Per score: one product-and-add, one exponential, half a maximum, one sum, half a conversion; the
 // running sums are rescaled only when a maximum has moved.
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams p, unsigned slots) {
-  constexpr int BQ = NW * 32, KT = 64, V = Elem<T>::kVec;
+__global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams p, unsigned slots, unsigned hop) {
+  constexpr int BQ = NW * 32, KT = sizeof(T) == 4 ? 32 : 64, V = Elem<T>::kVec;
   using KR = Rows<T, D, kRow>;
   using VR = Rows<T, D, kCol>;
   __shared__ __align__(1024) T buf[2][2][KT * D];          // [turn][k, v]
   extern __shared__ float line[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l = lane & 31;
-  const unsigned at = xcd_run(slots * p.heads);
+  const unsigned at = xcd_run(slots * p.heads, hop);
   const int head = at / slots;
   const Slot s = find_slot(p.offsets, p.n_seqs, p.total, BQ, at % slots);
   if (s.b < 0) return;
@@ -445,11 +449,11 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams 
     const T* sk = buf[t & 1][0];
     const T* sv = buf[t & 1][1];
     const int j0 = t * KT;
-    f32x16 x[2];
-    float shift[2] = {0.f, 0.f};         // a far tile's bias, added behind the product
+    f32x16 x[KT / 32];
+    float shift[KT / 32];                // a far tile's bias, added behind the product
     float top = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < KT / 32; ++u) {
       const int e0 = j0 + u * 32 - i0;
       shift[u] = c * scores<T, D, KR, 1>(x[u], sk, u * 32, fq, e0, p, line, mid + e0);
       if (j0 + u * 32 + 32 > len) {
@@ -471,7 +475,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams 
     }
     const float base = m == -INFINITY ? 0.f : m;       // a row of -inf alone: p = 0, not NaN
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < KT / 32; ++u) {
       const float off = shift[u] - base;
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][r], c, off));
@@ -738,7 +742,7 @@ __device__ __forceinline__ void add_diagonals(float* mine, int e0, const f32x16&
 // dq and the block's bucket sums.  Each wave: 32 queries, one per lane column; key tiles of 64 through LDS.  k is read along its rows (scores) and across them (ds k): one copy in LDS, in the order of the transposed reads, serves
 // both - the reads along it meet two by two on a bank.
 template <typename T, int D, int NW, bool DTABLE>
-__global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel(const AttnParams p, unsigned slots) {
+__global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel(const AttnParams p, unsigned slots, unsigned hop) {
   constexpr int BQ = NW * 32, KT = 64, V = Elem<T>::kVec;
   using R = Rows<T, D, kCol>;
   using RV = Rows<T, D, kRow>;
@@ -746,7 +750,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
   __shared__ float far[NW][2];
   extern __shared__ float line[];                          // 2 (R + margin) + 1, then NW * 2 lines of 2 (R + margin)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l = lane & 31;
-  const unsigned at = xcd_run(slots * p.heads);
+  const unsigned at = xcd_run(slots * p.heads, hop);
   const int head = at / slots;
   const unsigned slot = at % slots;
   const Slot s = find_slot(p.offsets, p.n_seqs, p.total, BQ, slot);
@@ -859,7 +863,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
 // dk and dv: each wave 32 keys, one per lane column; query tiles of 64 through LDS, q and dout once, in the order of the
 // transposed reads.
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kernel(const AttnParams p, unsigned slots) {
+__global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kernel(const AttnParams p, unsigned slots, unsigned hop) {
   constexpr int BQ = NW * 32, QT = 64, V = Elem<T>::kVec;
   using R = Rows<T, D, kCol>;
   using vec = typename Elem<T>::vec;
@@ -867,7 +871,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
   __shared__ __align__(16) float stat[2][2][QT];             // [turn][lse, delta]
   extern __shared__ float line[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l = lane & 31;
-  const unsigned at = xcd_run(slots * p.heads);
+  const unsigned at = xcd_run(slots * p.heads, hop);
   const int head = at / slots;
   const Slot s = find_slot(p.offsets, p.n_seqs, p.total, BQ, at % slots);
   if (s.b < 0) return;
