@@ -18,27 +18,66 @@ __device__ __forceinline__ float block_sum(float x, float* red) {
   return s;
 }
 
-// block: one sequence; a thread owns columns tid, tid + 256, ...
-template <typename T>
-__global__ __launch_bounds__(256) void mean_pool_kernel(const T* __restrict__ h, long long ld, const int64_t* __restrict__ offsets, long long total,
-                                                        long long dim, int normalize, float* __restrict__ y, float* __restrict__ inv_norm) {
-  __shared__ float red[4];
+// Block: one sequence.  The row's 16-byte pieces (VEC) or values go to neighbouring threads; what is left of the block takes further
+// rows at once, whose sums are joined in LDS, in order.  1024 texts of 3 to 128 rows of 768 bf16: 100 MB.
+template <typename T, bool VEC, int THREADS>
+__global__ __launch_bounds__(THREADS) void mean_pool_kernel(const T* __restrict__ h, long long ld, const int64_t* __restrict__ offsets, long long total,
+                                                            int dim, int normalize, float* __restrict__ y, float* __restrict__ inv_norm) {
+  constexpr int V = VEC ? Elem<T>::kVec : 1;
+  typedef T piece __attribute__((ext_vector_type(V)));
+  __shared__ float red[THREADS / 64];
+  __shared__ float join[THREADS * V];
   const long long b = blockIdx.x;
   const long long r0 = seq_edge(offsets, b, total);
   long long r1 = seq_edge(offsets, b + 1, total);
   if (r1 < r0) r1 = r0;
-  const float f = r1 > r0 ? 1.f / (float)(r1 - r0) : 0.f;
+  const int rows = (int)(r1 - r0);
+  const float f = rows ? 1.f / (float)rows : 0.f;
+  const int pieces = dim / V;
+  y += b * dim;
   float sq = 0.f;
-  for (long long c = threadIdx.x; c < dim; c += 256) {
-    float s = 0.f;
-    for (long long r = r0; r < r1; ++r) s += (float)h[r * ld + c];
-    s *= f;
-    y[b * dim + c] = s;
-    sq += s * s;
+  for (int p0 = 0; p0 < pieces; p0 += THREADS) {
+    const int n = pieces - p0 < THREADS ? pieces - p0 : THREADS, groups = THREADS / n, group = threadIdx.x / n, c = p0 + threadIdx.x % n;
+    float s[V] = {};
+    if (group < groups) {
+      const T* at = h + (r0 + group) * ld + (long long)c * V;
+      const long long step = groups * ld;
+      int r = group;
+      for (; r + 3 * groups < rows; r += 4 * groups, at += 4 * step) {
+        const piece x0 = *(const piece*)at, x1 = *(const piece*)(at + step), x2 = *(const piece*)(at + 2 * step), x3 = *(const piece*)(at + 3 * step);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[e] += ((float)x0[e] + (float)x1[e]) + ((float)x2[e] + (float)x3[e]);
+      }
+      for (; r < rows; r += groups, at += step) {
+        const piece x0 = *(const piece*)at;
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[e] += (float)x0[e];
+      }
+    }
+    if (groups > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < V; ++e) join[e * THREADS + threadIdx.x] = s[e];
+      __syncthreads();
+    }
+    if (group == 0) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        for (int k = 1; k < groups; ++k) s[e] += join[e * THREADS + k * n + threadIdx.x];
+        s[e] *= f;
+        y[(long long)c * V + e] = s[e];
+        sq += s[e] * s[e];
+      }
+    }
   }
   if (!normalize) return;
   const float inv = 1.f / fmaxf(sqrtf(block_sum(sq, red)), kTiny);
-  for (long long c = threadIdx.x; c < dim; c += 256) y[b * dim + c] *= inv;
+  for (int p0 = 0; p0 < pieces; p0 += THREADS) {       // the values that this thread wrote
+    const int n = pieces - p0 < THREADS ? pieces - p0 : THREADS, c = p0 + threadIdx.x;
+    if ((int)threadIdx.x < n)
+#pragma unroll
+      for (int e = 0; e < V; ++e) y[(long long)c * V + e] *= inv;
+  }
   if (inv_norm && threadIdx.x == 0) inv_norm[b] = inv;
 }
 
@@ -75,7 +114,13 @@ __global__ __launch_bounds__(256) void mean_pool_backward_kernel(const float* __
 
 template <typename T>
 hipError_t pool(const PoolArgs& a) {
-  mean_pool_kernel<T><<<(unsigned)a.n_seqs, 256, 0, a.st>>>((const T*)a.hidden, a.ld, a.offsets, a.total, a.dim, a.normalize, a.y, a.inv_norm);
+  const bool vec = ((uintptr_t)a.hidden & 15) == 0 && a.dim % Elem<T>::kVec == 0 && a.ld % Elem<T>::kVec == 0;
+  // few texts: more threads a text, for more rows under way
+  auto go = [&](auto kernel, int threads) {
+    kernel<<<(unsigned)a.n_seqs, threads, 0, a.st>>>((const T*)a.hidden, a.ld, a.offsets, a.total, (int)a.dim, a.normalize, a.y, a.inv_norm);
+  };
+  if (a.n_seqs < 512) vec ? go(mean_pool_kernel<T, true, 1024>, 1024) : go(mean_pool_kernel<T, false, 1024>, 1024);
+  else vec ? go(mean_pool_kernel<T, true, 256>, 256) : go(mean_pool_kernel<T, false, 256>, 256);
   return hipGetLastError();
 }
 template <typename T>

@@ -114,20 +114,29 @@ __device__ __forceinline__ Slot find_slot(const int64_t* __restrict__ offsets, l
   const int lane = threadIdx.x & 63;
   // the largest b in [0, n_seqs] with floor(begin_b / tile) + b <= slot; lo always satisfies it (b = 0 has slot 0)
   long long lo = 0, hi = n_seqs + 1;   // answer in [lo, hi)
+  int edge = 0, last = 0;              // lane's edge of the last round, and the lane of the answer: total is below 2^31
+  bool near = false;                   // the lane behind it holds the answer's end
   while (hi - lo > 1) {
     const long long step = (hi - lo + 63) >> 6;
     const long long b = lo + (long long)lane * step;
-    const bool ok = b < hi && (b == lo || seq_edge(offsets, b, total) / tile + b <= slot);
+    edge = b < hi ? (int)seq_edge(offsets, b, total) : 0;
+    const bool ok = b < hi && (b == lo || edge / tile + b <= slot);
     const unsigned long long m = __ballot(ok);
     // contents may be unordered: take the leading run of lanes that hold, which lane 0 always does
-    const int last = m == ~0ull ? 63 : __builtin_ctzll(~m) - 1;
+    last = m == ~0ull ? 63 : __builtin_ctzll(~m) - 1;
+    near = step == 1 && last < 63 && lo + last + 1 < hi;
     lo += (long long)last * step;
     hi = lo + step < hi ? lo + step : hi;
   }
   Slot s;
   s.b = lo;
-  s.begin = seq_edge(offsets, lo, total);
-  s.end = lo == n_seqs ? total : seq_edge(offsets, lo + 1, total);
+  if (near) {                          // one dependent load less
+    s.begin = __builtin_amdgcn_readlane(edge, last);
+    s.end = __builtin_amdgcn_readlane(edge, last + 1);
+  } else {
+    s.begin = seq_edge(offsets, lo, total);
+    s.end = lo == n_seqs ? total : seq_edge(offsets, lo + 1, total);
+  }
   if (s.end < s.begin) s.end = s.begin;
   const long long t = slot - (s.begin / tile + lo);
   if (t < 0 || t * tile >= s.end - s.begin) { s.b = -1; s.tile = 0; } else s.tile = (int)t;

@@ -16,6 +16,7 @@ the tensors' GPU, scratch comes from torch's allocator, nothing waits for the GP
 is no CPU fallback: tensors elsewhere raise ValueError.  torch.autocast does not reach in here: cast first."""
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
@@ -30,8 +31,14 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {"none": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
 
 
+_lib = None
+
+
 def _library():
-    return _capi.load_library()
+    global _lib
+    if _lib is None:
+        _lib = _capi.load_library()
+    return _lib
 
 
 def _chk(rc: int) -> None:
@@ -39,8 +46,13 @@ def _chk(rc: int) -> None:
         _capi.check(_library(), None, rc)
 
 
-def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+#: the current stream's handle without building a Stream object: a call on one text is over in a few microseconds
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_scratch(dt: int, m: int, n: int, k: int) -> int:
+    return _library().vdb_op_linear_workspace_bytes(dt, m, n, k)
 
 
 def _scratch(n: int, like: torch.Tensor) -> Optional[torch.Tensor]:
@@ -55,7 +67,7 @@ def _first(t, name: str) -> int:
     """Check a call's leading tensor; -> the C ABI's number of its type."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor; got {type(t).__name__}")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError(f"{name} must be on a GPU (there is no CPU fallback); got {t.device}")
     if t.dtype not in _DTYPES:
         raise ValueError(f"{name} must be float32, bfloat16 or float16; got {t.dtype}")
@@ -67,7 +79,7 @@ def _like(t, name: str, ref: torch.Tensor, shape) -> None:
         raise TypeError(f"{name} must be a torch.Tensor; got {type(t).__name__}")
     if t.device != ref.device or t.dtype != ref.dtype:
         raise ValueError(f"{name} must be {ref.dtype} on {ref.device}; got {t.dtype} on {t.device}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}; got {tuple(t.shape)}")
 
 
@@ -81,6 +93,8 @@ def _check_offsets(offsets, ref: torch.Tensor) -> torch.Tensor:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """A matrix whose rows are dense and do not overlap: itself, or a copy."""
+    if t.is_contiguous():
+        return t
     if t.stride(1) == 1 or t.shape[1] == 1:
         if t.stride(0) >= t.shape[1] or t.shape[0] <= 1:
             return t
@@ -104,11 +118,11 @@ def _linear_forward(x, weight, bias, residual, act: int, keep_z: bool):
     n = weight.shape[0]
     y = torch.empty((m, n), dtype=x.dtype, device=x.device)
     z = torch.empty_like(y) if keep_z else None
-    size = lib.vdb_op_linear_workspace_bytes(dt, m, n, k)
+    size = _linear_scratch(dt, m, n, k)
     ws = _scratch(size, x)
     _chk(lib.vdb_op_linear_dev(x.device.index, dt, x.data_ptr(), _ld(x), weight.data_ptr(), _ld(weight), _ptr(bias),
                                _ptr(residual), 0 if residual is None else _ld(residual), y.data_ptr(), n, _ptr(z), m, n, k, act,
-                               _ptr(ws), size, _stream(x)))
+                               _ptr(ws), size, _raw_stream(x.device.index)))
     return y, z
 
 
@@ -138,7 +152,7 @@ class _Linear(torch.autograd.Function):
             ws = _scratch(size, x)
             _chk(lib.vdb_op_linear_backward_dev(x.device.index, dt, dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), weight.data_ptr(),
                                                 _ld(weight), _ptr(z), _ptr(dx), _ptr(dw), _ptr(db), m, n, k, ctx.act, _ptr(ws), size,
-                                                _stream(x)))
+                                                _raw_stream(x.device.index)))
         return dx, dw, db, dy if need_r else None, None
 
 
@@ -160,21 +174,22 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
         raise ValueError("weight must be a tensor of shape [n, k] with n >= 1")
     n = weight.shape[0]
     _like(weight, "weight", x, (n, k))
-    lead = x.shape[:-1]
+    lead = tuple(x.shape[:-1])
     if bias is not None:
         _like(bias, "bias", x, (n,))
     if residual is not None:
         _like(residual, "residual", x, (*lead, n))
-    x2 = _rows(x.reshape(-1, k))
+    flat = x.dim() == 2
+    x2 = _rows(x if flat else x.reshape(-1, k))
     w2 = _rows(weight)
     b2 = None if bias is None else bias.contiguous()
-    r2 = None if residual is None else _rows(residual.reshape(-1, n))
+    r2 = None if residual is None else _rows(residual if flat else residual.reshape(-1, n))
     act = ACTIVATIONS[activation]
     if _wants_grad(x, weight, bias, residual):
         y = _Linear.apply(x2, w2, b2, r2, act)
     else:
         y = _linear_forward(x2, w2, b2, r2, act, False)[0]
-    return y.reshape(*lead, n)
+    return y if flat else y.reshape(*lead, n)
 
 
 # ---- attention ---------------------------------------------------------------------------------------------------------
@@ -194,7 +209,7 @@ def _attention_forward(qkv, table, offsets, scale, max_distance, keep_lse: bool)
     total, _, heads, d = qkv.shape
     out = torch.empty((total, heads, d), dtype=qkv.dtype, device=qkv.device)
     lse = torch.empty((heads, total), dtype=torch.float32, device=qkv.device) if keep_lse else None
-    _chk(lib.vdb_op_attention_dev(*_attention_args(qkv, table, offsets, scale, max_distance), out.data_ptr(), _ptr(lse), _stream(qkv)))
+    _chk(lib.vdb_op_attention_dev(*_attention_args(qkv, table, offsets, scale, max_distance), out.data_ptr(), _ptr(lse), _raw_stream(qkv.device.index)))
     return out, lse
 
 
@@ -220,7 +235,7 @@ class _BucketedAttention(torch.autograd.Function):
         base, step = dqkv.data_ptr(), heads * d * dqkv.element_size()
         _chk(lib.vdb_op_attention_backward_dev(*_attention_args(qkv, table, offsets, ctx.scale, ctx.max_distance), out.data_ptr(), lse.data_ptr(),
                                                dout.data_ptr(), base, base + step, base + 2 * step, 3 * heads * d, d, _ptr(dtable),
-                                               _ptr(ws), size, _stream(qkv)))
+                                               _ptr(ws), size, _raw_stream(qkv.device.index)))
         return dqkv if ctx.needs_input_grad[0] else None, dtable, None, None, None
 
 
@@ -259,7 +274,7 @@ def _pool_forward(hidden, offsets, normalize: bool, keep: bool):
     y = torch.empty((n, dim), dtype=torch.float32, device=hidden.device)
     inv = torch.empty((n,), dtype=torch.float32, device=hidden.device) if keep and normalize else None
     _chk(lib.vdb_op_mean_pool_dev(hidden.device.index, _DTYPES[hidden.dtype], hidden.data_ptr(), _ld(hidden), offsets.data_ptr(), n, total, dim,
-                                  int(normalize), y.data_ptr(), _ptr(inv), _stream(hidden)))
+                                  int(normalize), y.data_ptr(), _ptr(inv), _raw_stream(hidden.device.index)))
     return y, inv
 
 
@@ -279,7 +294,7 @@ class _MeanPool(torch.autograd.Function):
         dy = dy.contiguous()
         dh = torch.empty((ctx.total, dim), dtype=ctx.dtype, device=y.device)
         _chk(_library().vdb_op_mean_pool_backward_dev(y.device.index, _DTYPES[ctx.dtype], dy.data_ptr(), y.data_ptr(), _ptr(inv), offsets.data_ptr(), n,
-                                                      ctx.total, dim, int(ctx.normalize), dh.data_ptr(), _stream(y)))
+                                                      ctx.total, dim, int(ctx.normalize), dh.data_ptr(), _raw_stream(y.device.index)))
         return dh, None, None
 
 
