@@ -138,7 +138,7 @@ hipError_t act_grad(const ActGradArgs& a) {
   act_grad_kernel<T, ACT><<<grid, 256, 0, a.st>>>((const T*)a.dy, a.lddy, (const T*)a.z, (T*)a.dz, a.db ? a.partial : nullptr, a.m, a.n, rows);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !a.db) return e;
-  col_join_kernel<T><<<(unsigned)cdiv(a.n, 256), 256, 0, a.st>>>(a.partial, parts, a.n, (T*)a.db);
+  col_join_kernel<T><<<(unsigned)cdiv(a.n, 32), 256, 0, a.st>>>(a.partial, parts, a.n, (T*)a.db);
   return hipGetLastError();
 }
 

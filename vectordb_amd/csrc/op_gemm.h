@@ -516,12 +516,19 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy,
   if (wave == 0 && j < n) part[(long long)blockIdx.y * n + j] = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
 }
 
+// 32 columns a block; eight threads a column take the parts in turn and are joined in order, in 64 bits
 template <typename T>
 __global__ __launch_bounds__(256) void col_join_kernel(const float* __restrict__ part, int parts, long long n, T* __restrict__ db) {
-  const long long j = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (j >= n) return;
+  __shared__ double red[8][32];
+  const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
+  const long long j = (long long)blockIdx.x * 32 + c;
   double s = 0.0;
-  for (int i = 0; i < parts; ++i) s += part[(long long)i * n + j];
+  if (j < n)
+    for (int i = g; i < parts; i += 8) s += part[(long long)i * n + j];
+  red[g][c] = s;
+  __syncthreads();
+  if (g || j >= n) return;
+  for (int i = 1; i < 8; ++i) s += red[i][c];
   db[j] = (T)(float)s;
 }
 
