@@ -56,17 +56,18 @@ int vdb_op_linear_backward_dev(int device, int dtype, const void* dy, int64_t ld
  * with n >= near (max_distance/near)^(i/(half-near)) (compared in whole numbers); + half where e > 0.  This is the
  * bidirectional bucketing of the reference's embedding model (32 buckets, max_distance 128).
  * q, k, v: token stride ld_t, head stride ld_h, dense head rows of head_dim.  out: dense [total][heads][head_dim].
- * lse (may be NULL): fp32 [heads][total], log2 of the softmax denominators, kept for the backward pass. */
+ * Kept for the backward pass, each may be NULL: lse fp32 [heads][total], log2 of the softmax denominators; rest, of out's type and
+ * shape, what the rounding of out left (16-bit types: the gradients need rowsum(dout out) closer than that rounding). */
 int vdb_op_attention_dev(int device, int dtype, const void* q, const void* k, const void* v, int64_t ld_t, int64_t ld_h,
                          const void* table, int n_buckets, int max_distance, const int64_t* offsets, int64_t n_seqs,
-                         int64_t total, int heads, int head_dim, float scale, void* out, float* lse, void* stream);
+                         int64_t total, int heads, int head_dim, float scale, void* out, void* rest, float* lse, void* stream);
 
 /* Gradients for dout (dense, like out): dq, dk, dv (strides gld_t, gld_h) and dtable [n_buckets][heads] (dense; NULL = not
- * wanted).  ds = p (dout v^T - rowsum(dout out)) is rounded to the operands' type before the products with k and q. */
+ * wanted).  ds = p (dout v^T - rowsum(dout (out + rest))) is rounded to the operands' type before the products with k and q. */
 int64_t vdb_op_attention_backward_workspace_bytes(int dtype, int64_t n_seqs, int64_t total, int heads, int head_dim, int n_buckets);
 int vdb_op_attention_backward_dev(int device, int dtype, const void* q, const void* k, const void* v, int64_t ld_t, int64_t ld_h,
                                   const void* table, int n_buckets, int max_distance, const int64_t* offsets, int64_t n_seqs,
-                                  int64_t total, int heads, int head_dim, float scale, const void* out, const float* lse,
+                                  int64_t total, int heads, int head_dim, float scale, const void* out, const void* rest, const float* lse,
                                   const void* dout, void* dq, void* dk, void* dv, int64_t gld_t, int64_t gld_h, void* dtable,
                                   void* workspace, int64_t workspace_bytes, void* stream);
 

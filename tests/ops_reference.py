@@ -108,6 +108,7 @@ def attention(qkv, table, ends, scale, max_distance, dout=None):
             ep = 2 * es + (n + 16) * E                                   # relative error of p in 32 bits
             o = p @ v
             ob = (ep + p16 + (n + 4) * E) * (p @ v.abs())
+            kept = ob + p16 * u * o.abs() + (2.0 ** -25 if t == torch.float16 else 0)      # out and the rest of its rounding, rounded too
             ob = ob + u * (o.abs() + ob) + tiny(t)
             out[lo:hi, h], outb[lo:hi, h] = o, ob
             if dout is None:
@@ -115,7 +116,7 @@ def attention(qkv, table, ends, scale, max_distance, dout=None):
             g = dout[lo:hi, h].double()
             dp = g @ v.t()
             delta = (g * o).sum(1, keepdim=True)
-            eb = (d + 4) * E * (g.abs() @ v.abs().t()) + (g.abs() * ob).sum(1, keepdim=True) + (d + 4) * E * (g * o).abs().sum(1, keepdim=True)
+            eb = (d + 4) * E * (g.abs() @ v.abs().t()) + (g.abs() * kept).sum(1, keepdim=True) + (d + 4) * E * (g * o).abs().sum(1, keepdim=True)
             ds = p * (dp - delta)
             d32 = p * (eb + (ep + 2 * E) * ((dp - delta).abs() + eb))
             # one product of p and ds rounded, with the 16-bit type's own floor: fp16 lifts ds by a power of two, whose floor is

@@ -76,7 +76,7 @@ def test_linear_backward_refusals(hip_lib):
 
 def test_attention_refusals(hip_lib):
     def call(dtype=1, q=P, table=P, nb=32, dist=128, off=P, seqs=2, total=10, heads=2, d=16, scale=0.25, out=P, ld_t=96):
-        return hip_lib.vdb_op_attention_dev(0, dtype, q, P, P, ld_t, 16, table, nb, dist, off, seqs, total, heads, d, scale, out, None, None)
+        return hip_lib.vdb_op_attention_dev(0, dtype, q, P, P, ld_t, 16, table, nb, dist, off, seqs, total, heads, d, scale, out, None, None, None)
     _refused(hip_lib, call(dtype=5), "dtype")
     for name, bad in (("q", None), ("table", None), ("off", None), ("out", None)):
         _refused(hip_lib, call(**{name: bad}), "NULL")
@@ -95,9 +95,9 @@ def test_attention_refusals(hip_lib):
     _refused(hip_lib, call(ld_t=-1), "stride")
     _refused(hip_lib, call(seqs=1 << 29, heads=1024), "too many")
     assert call(total=0, q=None, table=None, off=None, out=None) == 0
-    rc = hip_lib.vdb_op_attention_backward_dev(0, 1, P, P, P, 96, 16, P, 32, 128, P, 2, 10, 2, 16, 0.25, P, P, P, P, P, P, 96, 16, P, P, 1, None)
+    rc = hip_lib.vdb_op_attention_backward_dev(0, 1, P, P, P, 96, 16, P, 32, 128, P, 2, 10, 2, 16, 0.25, P, None, P, P, P, P, P, 96, 16, P, P, 1, None)
     _refused(hip_lib, rc, "workspace")
-    rc = hip_lib.vdb_op_attention_backward_dev(0, 1, P, P, P, 96, 16, P, 32, 128, P, 2, 10, 2, 16, 0.25, P, None, P, P, P, P, 96, 16, P, P, 1 << 30, None)
+    rc = hip_lib.vdb_op_attention_backward_dev(0, 1, P, P, P, 96, 16, P, 32, 128, P, 2, 10, 2, 16, 0.25, P, None, None, P, P, P, P, 96, 16, P, P, 1 << 30, None)
     _refused(hip_lib, rc, "NULL")
 
 

@@ -104,9 +104,9 @@ def _declare_ops(lib: C.CDLL) -> C.CDLL:
     lib.vdb_op_linear_dev.argtypes = [i32, i32, vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, i64, i64, i64, i32, vp, i64, vp]
     lib.vdb_op_linear_backward_workspace_bytes.argtypes = [i32, i64, i64, i64, i32]
     lib.vdb_op_linear_backward_dev.argtypes = [i32, i32, vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, i64, i64, i64, i32, vp, i64, vp]
-    lib.vdb_op_attention_dev.argtypes = [i32, i32, vp, vp, vp, i64, i64, vp, i32, i32, vp, i64, i64, i32, i32, f32, vp, vp, vp]
+    lib.vdb_op_attention_dev.argtypes = [i32, i32, vp, vp, vp, i64, i64, vp, i32, i32, vp, i64, i64, i32, i32, f32, vp, vp, vp, vp]
     lib.vdb_op_attention_backward_workspace_bytes.argtypes = [i32, i64, i64, i32, i32, i32]
-    lib.vdb_op_attention_backward_dev.argtypes = [i32, i32, vp, vp, vp, i64, i64, vp, i32, i32, vp, i64, i64, i32, i32, f32, vp, vp, vp,
+    lib.vdb_op_attention_backward_dev.argtypes = [i32, i32, vp, vp, vp, i64, i64, vp, i32, i32, vp, i64, i64, i32, i32, f32, vp, vp, vp, vp,
                                                   vp, vp, vp, i64, i64, vp, vp, i64, vp]
     lib.vdb_op_mean_pool_dev.argtypes = [i32, i32, vp, i64, vp, i64, i64, i64, i32, vp, vp, vp]
     lib.vdb_op_mean_pool_backward_dev.argtypes = [i32, i32, vp, vp, vp, vp, i64, i64, i64, i32, vp, vp]

@@ -18,12 +18,12 @@ AttnParams params(const AttnArgs& a, int elem) {
   AttnParams p{};
   p.q = a.q; p.k = a.k; p.v = a.v; p.ld_t = a.ld_t; p.ld_h = a.ld_h; p.table = a.table; p.n_buckets = a.n_buckets;
   p.offsets = a.offsets; p.n_seqs = a.n_seqs; p.total = a.total; p.heads = a.heads; p.d = a.d; p.scale = a.scale;
-  p.out = a.out; p.lse = a.lse; p.dout = a.dout; p.dq = a.dq; p.dk = a.dk; p.dv = a.dv; p.gld_t = a.gld_t; p.gld_h = a.gld_h;
+  p.out = a.out; p.rest = a.rest; p.lse = a.lse; p.dout = a.dout; p.dq = a.dq; p.dk = a.dk; p.dv = a.dv; p.gld_t = a.gld_t; p.gld_h = a.gld_h;
   p.bk = a.bk;
   p.reach = a.bk.n_steps ? a.bk.step[a.bk.n_steps - 1] : a.bk.near;
   const int64_t v = 16 / elem;
   auto al = [](const void* x) { return ((uintptr_t)x & 15) == 0; };
-  p.vec = al(a.q) && al(a.k) && al(a.v) && al(a.out) && al(a.dout) && al(a.dq) && al(a.dk) && al(a.dv) && a.d % v == 0 && a.ld_t % v == 0 &&
+  p.vec = al(a.q) && al(a.k) && al(a.v) && al(a.out) && al(a.rest) && al(a.dout) && al(a.dq) && al(a.dk) && al(a.dv) && a.d % v == 0 && a.ld_t % v == 0 &&
           a.ld_h % v == 0 && a.gld_t % v == 0 && a.gld_h % v == 0 && a.ld_t < ((int64_t)1 << 22);
   return p;
 }

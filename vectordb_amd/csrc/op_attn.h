@@ -20,7 +20,7 @@ struct AttnParams {
   const void* table; int n_buckets;
   const int64_t* offsets; long long n_seqs, total;
   int heads, d; float scale;
-  void* out; float* lse;
+  void* out; void* rest; float* lse;
   const void* dout; void *dq, *dk, *dv; long long gld_t, gld_h;
   float* delta; const unsigned* peak; float* part;   // peak: [2][heads][n_seqs] largest |dout| and |v| (fp16 only)
   int vec;        // q, k, v, out, dout, gradients: 16-byte rows
@@ -138,8 +138,14 @@ __device__ __forceinline__ void trans_times(f32x16 (&acc)[DP / 32], const T* st,
   }
 }
 
+// A scaled sum as it is stored, or (LOW) what that rounding left of it
+template <typename T, bool LOW> __device__ __forceinline__ T rounded(float x) {
+  const T t = (T)x;
+  return LOW ? (T)(x - (float)t) : t;
+}
+
 // C registers [DP / 32] with C column = a token row: store columns [0, d) of that row, scaled
-template <typename T, int DP>
+template <typename T, int DP, bool LOW = false>
 __device__ __forceinline__ void store_cols(T* row, const f32x16 (&acc)[DP / 32], float f, int d, int vec_ok) {
   const int half = (threadIdx.x & 63) >> 5;
 #pragma unroll
@@ -147,7 +153,9 @@ __device__ __forceinline__ void store_cols(T* row, const f32x16 (&acc)[DP / 32],
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int c = db * 32 + 8 * g + 4 * half;
-      T x[4] = {(T)(acc[db][4 * g] * f), (T)(acc[db][4 * g + 1] * f), (T)(acc[db][4 * g + 2] * f), (T)(acc[db][4 * g + 3] * f)};
+      T x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = rounded<T, LOW>(acc[db][4 * g + e] * f);
       if (vec_ok && c + 4 <= d) {
         if constexpr (sizeof(T) == 2) *(i32x2*)(row + c) = *(i32x2*)x; else *(i32x4*)(row + c) = *(i32x4*)x;
       } else {
@@ -239,7 +247,9 @@ __global__ __launch_bounds__(NW * 64) void attention_any_kernel(const AttnParams
   }
   if (i >= len) return;
   l += __shfl_xor(l, 32, 64);
-  store_cols<T, DP>((T*)p.out + (s.begin + i) * hd + (long long)head * p.d, acc, l > 0.f || l != l ? 1.f / l : 0.f, p.d, p.vec);
+  const float f = l > 0.f || l != l ? 1.f / l : 0.f;
+  store_cols<T, DP>((T*)p.out + (s.begin + i) * hd + (long long)head * p.d, acc, f, p.d, p.vec);
+  if (p.rest) store_cols<T, DP, true>((T*)p.rest + (s.begin + i) * hd + (long long)head * p.d, acc, f, p.d, p.vec);
   // +inf where nothing was left of the row: the backward pass' exp2(s - lse) is 0 there
   if (p.lse && lane < 32) p.lse[(long long)head * p.total + s.begin + i] = l > 0.f || l != l ? m + log2f(l) : INFINITY;
 }
@@ -362,7 +372,7 @@ __device__ __forceinline__ float scores(f32x16& x, const T* s, int r0, const typ
 }
 
 // C registers -> D / 32 column blocks of the wave's 32 rows, through LDS of the wave's own, as whole rows
-template <typename T, int D>
+template <typename T, int D, bool LOW = false>
 __device__ __forceinline__ void store_turned(T* mine, T* dst, long long ld, const f32x16 (&acc)[D / 32], float f, int rows) {
   using R = Rows<T, D, kRow>;
   typedef T vec4 __attribute__((ext_vector_type(4)));
@@ -374,7 +384,7 @@ __device__ __forceinline__ void store_turned(T* mine, T* dst, long long ld, cons
       const int c = db * 32 + 8 * g + 4 * half;
       vec4 o;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = (T)(acc[db][4 * g + e] * f);
+      for (int e = 0; e < 4; ++e) o[e] = rounded<T, LOW>(acc[db][4 * g + e] * f);
       *(vec4*)(mine + l * D + (((c / R::V) ^ R::swz(l)) * R::V) + (c & (R::V - 1))) = o;
     }
   asm volatile("" ::: "memory");       // a wave's LDS operations keep their order
@@ -489,7 +499,9 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams 
   sum += __shfl_xor(sum, 32, 64);
   const bool any = sum > 0.f || sum != sum;
   T* mine = &buf[0][0][0] + wave * (32 * D);
-  store_turned<T, D>(mine, (T*)p.out + (s.begin + i0) * hd + (long long)head * D, hd, acc, any ? 1.f / sum : 0.f, len - i0);
+  const float f = any ? 1.f / sum : 0.f;
+  store_turned<T, D>(mine, (T*)p.out + (s.begin + i0) * hd + (long long)head * D, hd, acc, f, len - i0);
+  if (p.rest) store_turned<T, D, true>(mine, (T*)p.rest + (s.begin + i0) * hd + (long long)head * D, hd, acc, f, len - i0);
   if (p.lse && lane < 32 && i0 + l < len) p.lse[(long long)head * p.total + s.begin + i0 + l] = any ? m + __log2f(sum) : INFINITY;
 }
 
@@ -519,7 +531,7 @@ __device__ __forceinline__ void fold_buckets(const AttnParams& p, float* hist, c
 }
 
 // ---- backward -------------------------------------------------------------------------------------------------------------
-// delta[h][t] = sum_d dout out (the general kernels'; attention_dq_kernel has its own); fp16 also the largest |dout| and |v| of each sequence and head (bits of non-negative
+// delta[h][t] = sum_d dout (out + rest) (the general kernels'; attention_dq_kernel has its own); fp16 also the largest |dout| and |v| of each sequence and head (bits of non-negative
 // floats order like integers, so the atomic maximum does not depend on the order of arrival).
 template <typename T, bool PEAK>
 __global__ __launch_bounds__(256) void attention_delta_kernel(const AttnParams p, unsigned* peak) {
@@ -536,7 +548,7 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(const AttnParams p
     const T* v = (const T*)p.v + t * p.ld_t + head * p.ld_h;
     float x = 0.f;
     for (int c = lane; c < p.d; c += 64) {
-      x += (float)o[c] * (float)g[c];
+      x += ((float)o[c] + (p.rest ? (float)((const T*)p.rest)[(t * p.heads + head) * p.d + c] : 0.f)) * (float)g[c];
       if (PEAK) { po = fmaxf(po, fabsf((float)g[c])); pv = fmaxf(pv, fabsf((float)v[c])); }
     }
     for (int k = 32; k; k >>= 1) x += __shfl_xor(x, k, 64);
@@ -792,8 +804,10 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
 #pragma unroll
     for (int x = 0; x < D / (2 * V); ++x) {
       const vec fo = *(const vec*)(o + x * 2 * V);
+      vec fr = {};
+      if (p.rest) fr = *(const vec*)((const T*)p.rest + (o - (const T*)p.out) + x * 2 * V);
 #pragma unroll
-      for (int e = 0; e < V; ++e) delta += (float)fo[e] * (float)fg[x][e];
+      for (int e = 0; e < V; ++e) delta += ((float)fo[e] + (float)fr[e]) * (float)fg[x][e];
     }
     delta += __shfl_xor(delta, 32, 64);
     if (lane < 32 && i0 + l < len) p.delta[row] = delta;

@@ -39,7 +39,7 @@ struct AttnArgs {
   const void* table; int n_buckets; Buckets bk;
   const int64_t* offsets; int64_t n_seqs, total;
   int heads, d; float scale;
-  void* out; float* lse;
+  void* out; void* rest; float* lse;     // rest: what the rounding of out left, or nullptr
   // backward
   const void* dout; void *dq, *dk, *dv; int64_t gld_t, gld_h; void* dtable;
   float* delta; float* gscale; float* part;    // workspace pieces

@@ -178,7 +178,7 @@ int vdb_op_linear_backward_dev(int device, int dtype, const void* dy, int64_t ld
 
 int vdb_op_attention_dev(int device, int dtype, const void* q, const void* k, const void* v, int64_t ld_t, int64_t ld_h, const void* table,
                          int n_buckets, int max_distance, const int64_t* offsets, int64_t n_seqs, int64_t total, int heads, int head_dim,
-                         float scale, void* out, float* lse, void* stream) {
+                         float scale, void* out, void* rest, float* lse, void* stream) {
   const int rc = check_attention(dtype, q, k, v, ld_t, ld_h, table, n_buckets, max_distance, offsets, n_seqs, total, heads, head_dim, scale);
   if (rc) return rc;
   if (total == 0) return VDB_OK;
@@ -186,7 +186,7 @@ int vdb_op_attention_dev(int device, int dtype, const void* q, const void* k, co
   ON_DEVICE("attention");
   AttnArgs a{};
   a.q = q; a.k = k; a.v = v; a.ld_t = ld_t; a.ld_h = ld_h; a.table = table; a.n_buckets = n_buckets; a.bk = make_buckets(n_buckets, max_distance);
-  a.offsets = offsets; a.n_seqs = n_seqs; a.total = total; a.heads = heads; a.d = head_dim; a.scale = scale; a.out = out; a.lse = lse;
+  a.offsets = offsets; a.n_seqs = n_seqs; a.total = total; a.heads = heads; a.d = head_dim; a.scale = scale; a.out = out; a.rest = rest; a.lse = lse;
   a.st = (hipStream_t)stream;
   const hipError_t e = launch_attention(dtype, a);
   return e == hipSuccess ? VDB_OK : hip_fail("attention", e);
@@ -199,7 +199,7 @@ int64_t vdb_op_attention_backward_workspace_bytes(int dtype, int64_t n_seqs, int
 
 int vdb_op_attention_backward_dev(int device, int dtype, const void* q, const void* k, const void* v, int64_t ld_t, int64_t ld_h,
                                   const void* table, int n_buckets, int max_distance, const int64_t* offsets, int64_t n_seqs, int64_t total,
-                                  int heads, int head_dim, float scale, const void* out, const float* lse, const void* dout, void* dq, void* dk,
+                                  int heads, int head_dim, float scale, const void* out, const void* rest, const float* lse, const void* dout, void* dq, void* dk,
                                   void* dv, int64_t gld_t, int64_t gld_h, void* dtable, void* workspace, int64_t workspace_bytes, void* stream) {
   const int rc = check_attention(dtype, q, k, v, ld_t, ld_h, table, n_buckets, max_distance, offsets, n_seqs, total, heads, head_dim, scale);
   if (rc) return rc;
@@ -210,7 +210,7 @@ int vdb_op_attention_backward_dev(int device, int dtype, const void* q, const vo
   ON_DEVICE("attention_backward");
   AttnArgs a{};
   a.q = q; a.k = k; a.v = v; a.ld_t = ld_t; a.ld_h = ld_h; a.table = table; a.n_buckets = n_buckets; a.bk = make_buckets(n_buckets, max_distance);
-  a.offsets = offsets; a.n_seqs = total ? n_seqs : 0; a.total = total; a.heads = heads; a.d = head_dim; a.scale = scale; a.out = (void*)out; a.lse = (float*)lse;
+  a.offsets = offsets; a.n_seqs = total ? n_seqs : 0; a.total = total; a.heads = heads; a.d = head_dim; a.scale = scale; a.out = (void*)out; a.rest = (void*)rest; a.lse = (float*)lse;
   a.dout = dout; a.dq = dq; a.dk = dk; a.dv = dv; a.gld_t = gld_t; a.gld_h = gld_h; a.dtable = dtable; a.st = (hipStream_t)stream;
   const hipError_t e = launch_attention_backward(dtype, a, (char*)workspace);
   return e == hipSuccess ? VDB_OK : hip_fail("attention_backward", e);

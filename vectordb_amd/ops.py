@@ -204,27 +204,28 @@ def _attention_args(qkv, table, offsets, scale, max_distance):
             offsets.data_ptr(), offsets.shape[0] - 1, total, heads, d, scale)
 
 
-def _attention_forward(qkv, table, offsets, scale, max_distance, keep_lse: bool):
+def _attention_forward(qkv, table, offsets, scale, max_distance, keep: bool):
     lib = _library()
     total, _, heads, d = qkv.shape
     out = torch.empty((total, heads, d), dtype=qkv.dtype, device=qkv.device)
-    lse = torch.empty((heads, total), dtype=torch.float32, device=qkv.device) if keep_lse else None
-    _chk(lib.vdb_op_attention_dev(*_attention_args(qkv, table, offsets, scale, max_distance), out.data_ptr(), _ptr(lse), _raw_stream(qkv.device.index)))
-    return out, lse
+    lse = torch.empty((heads, total), dtype=torch.float32, device=qkv.device) if keep else None
+    rest = torch.empty_like(out) if keep and qkv.dtype != torch.float32 else None
+    _chk(lib.vdb_op_attention_dev(*_attention_args(qkv, table, offsets, scale, max_distance), out.data_ptr(), _ptr(rest), _ptr(lse), _raw_stream(qkv.device.index)))
+    return out, rest, lse
 
 
 class _BucketedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, table, offsets, scale, max_distance):
-        out, lse = _attention_forward(qkv, table, offsets, scale, max_distance, True)
+        out, rest, lse = _attention_forward(qkv, table, offsets, scale, max_distance, True)
         ctx.scale, ctx.max_distance = scale, max_distance
-        ctx.save_for_backward(qkv, table, offsets, out, lse)
+        ctx.save_for_backward(qkv, table, offsets, out, rest, lse)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        qkv, table, offsets, out, lse = ctx.saved_tensors
+        qkv, table, offsets, out, rest, lse = ctx.saved_tensors
         lib = _library()
         total, _, heads, d = qkv.shape
         dout = dout.contiguous()
@@ -233,7 +234,7 @@ class _BucketedAttention(torch.autograd.Function):
         size = lib.vdb_op_attention_backward_workspace_bytes(_DTYPES[qkv.dtype], offsets.shape[0] - 1, total, heads, d, table.shape[0])
         ws = _scratch(size, qkv)
         base, step = dqkv.data_ptr(), heads * d * dqkv.element_size()
-        _chk(lib.vdb_op_attention_backward_dev(*_attention_args(qkv, table, offsets, ctx.scale, ctx.max_distance), out.data_ptr(), lse.data_ptr(),
+        _chk(lib.vdb_op_attention_backward_dev(*_attention_args(qkv, table, offsets, ctx.scale, ctx.max_distance), out.data_ptr(), _ptr(rest), lse.data_ptr(),
                                                dout.data_ptr(), base, base + step, base + 2 * step, 3 * heads * d, d, _ptr(dtable),
                                                _ptr(ws), size, _raw_stream(qkv.device.index)))
         return dqkv if ctx.needs_input_grad[0] else None, dtable, None, None, None
