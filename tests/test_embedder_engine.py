@@ -62,7 +62,7 @@ def test_hip_engine_gives_the_models_vectors(tmp_path, hip_lib, hidden):
     assert float((got - want).abs().max()) < 2e-6
     assert torch.equal(hip.embed_device(TEXTS), got)
     assert torch.equal(got[0], got[7]) and np.array_equal(np.stack(hip(TEXTS[:1]))[0], hip.embed_device(TEXTS[:1])[0].cpu().numpy())
-    assert hip.embed_device([]).shape == (0, hidden)
+    assert hip.embed_device([]).shape == (0, hidden) and hip.encode([]).shape == (0, hidden)
     for amp, tol in (("bf16", 1e-2), ("fp16", 2e-3)):
         low = MPNetEmbedder(d, device="cuda:0", autocast=amp, engine="hip").embed_device(TEXTS)
         assert low.dtype == torch.float32 and float((low - want).abs().max()) < tol

@@ -86,7 +86,8 @@ def test_linear_gradients(ops, dtype, name, m, n, k):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m,n,k,name", [(1000, 776, 776, "none"), (2049, 1400, 72, "gelu"), (8200, 4104, 72, "none"), (8200, 4104, 136, "gelu_tanh"), (2100, 1409, 200, "relu"),
-                                        (16385, 2056, 64, "gelu"), (5000, 40, 1000, "none")])
+                                        (16385, 2056, 64, "gelu"), (5000, 40, 1000, "none"),
+                                        (500, 768, 1032, "gelu"), (1001, 768, 2312, "relu")])
 def test_linear_forward_large(ops, dtype, m, n, k, name):
     """Sizes that take each of the tiled kernels, with ragged edges in all three dimensions (64-bit form on the GPU)."""
     g = torch.Generator(device="cuda").manual_seed(m + n + k)
@@ -221,6 +222,61 @@ def test_attention_buckets(ops, dtype, n_buckets, max_distance):
     lq, lt = qkv.cuda().requires_grad_(), table.cuda().requires_grad_()
     out = ops.bucketed_attention(lq, lt, off, scale=0.3, max_distance=max_distance)
     hold([out, *torch.autograd.grad(out, [lq, lt], dout.cuda())], want, f"{n_buckets} {max_distance}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_attention_widest_buckets(ops, dtype, d):
+    """The largest table and distance with the widest heads: the most LDS a block can ask for."""
+    t = DT[dtype]
+    g = torch.Generator().manual_seed(d)
+    qkv, table, dout = rnd(g, 300, 3, 1, d, dtype=t), rnd(g, 128, 1, dtype=t), rnd(g, 300, 1, d, dtype=t)
+    off = offsets_of([260, 40])
+    want = ref.attention(qkv, table, off.tolist(), d ** -0.5, 512, dout)
+    lq, lt = qkv.cuda().requires_grad_(), table.cuda().requires_grad_()
+    out = ops.bucketed_attention(lq, lt, off, max_distance=512)
+    hold([out, *torch.autograd.grad(out, [lq, lt], dout.cuda())], want, dtype)
+
+
+def test_what_is_refused(ops):
+    """Arguments that do not fit together raise before any launch."""
+    x, w = torch.zeros(4, 8, device="cuda"), torch.zeros(6, 8, device="cuda")
+    off = torch.zeros(2, dtype=torch.int64, device="cuda")
+    for args, kw, text in (((x, w.half()), {}, "weight"), ((x, w[:, :4]), {}, "weight"), ((x, w[0]), {}, "weight"), ((x, w, x), {}, "bias"),
+                           ((x, w, torch.zeros(6)), {}, "bias"), ((x, w), dict(residual=x), "residual"), ((x, w), dict(activation="tanh"), "activation"),
+                           ((x.double(), w.double()), {}, "float32"), ((x.cpu(), w), {}, "GPU"), ((x[:, :0], w[:, :0]), {}, "k >= 1")):
+        with pytest.raises(ValueError, match=text):
+            ops.linear(*args, **kw)
+    with pytest.raises(TypeError):
+        ops.linear(x, w, bias=1.0)
+    q, t = torch.zeros(5, 3, 2, 16, device="cuda"), torch.zeros(32, 2, device="cuda")
+    for args, kw, text in (((q[:, :2], t, off), {}, "qkv"), ((torch.zeros(5, 3, 2, 136, device="cuda"), t, off), {}, "qkv"), ((q, t[:, :1], off), {}, "table"),
+                           ((q, t.bfloat16(), off), {}, "table"), ((q, t[0], off), {}, "table"), ((q, t, off.int()), {}, "offsets"),
+                           ((q, t, off.cpu()), {}, "offsets"), ((q, t, off[:0]), {}, "offsets"), ((q, t, off[None]), {}, "offsets")):
+        with pytest.raises(ValueError, match=text):
+            ops.bucketed_attention(*args, **kw)
+    from vectordb_amd import VdbError
+    for kw, text in ((dict(scale=0.0), "scale"), (dict(scale=math.nan), "scale"), (dict(max_distance=8), "max_distance"), (dict(max_distance=513), "max_distance")):
+        with pytest.raises(VdbError, match=text):
+            ops.bucketed_attention(q, t, off, **kw)
+    for n in (2, 33, 130):
+        with pytest.raises(VdbError, match="n_buckets"):
+            ops.bucketed_attention(q, torch.zeros(n, 2, device="cuda"), off)
+    for args, text in (((x[0], off), "hidden"), ((x, off.int()), "offsets"), ((x, off.cpu()), "offsets"), ((x.to(torch.int32), off), "float32")):
+        with pytest.raises(ValueError, match=text):
+            ops.mean_pool(*args)
+    # a second derivative is refused, not wrong
+    lx = x.clone().requires_grad_()
+    first, = torch.autograd.grad(ops.linear(lx, w, activation="gelu").sum(), [lx], create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(first.sum(), [lx])
+    # an operand changed between the two passes is noticed
+    lw = w.clone().requires_grad_()
+    y = ops.linear(lx, lw, activation="gelu")
+    with torch.no_grad():
+        lw.add_(1)
+    with pytest.raises(RuntimeError, match="modified"):
+        y.sum().backward()
 
 
 @pytest.mark.parametrize("dtype", TYPES)

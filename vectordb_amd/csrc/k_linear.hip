@@ -10,15 +10,20 @@ int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Which kernel serves a product: one rule on sizes and alignment, for the launch and for the size of its scratch.
 //   any    a row or a width that is no whole number of 16-byte pieces;
-//   few    (forward) fewer than 128 tiles of 64 x 64: there a block a tile leaves most of the chip idle.  1000 x 768 from 768 in
-//          bf16: 192 tiles 7.6 us, few 8.3; 200 x 768: 48 tiles 7.0, few 5.1; 14 x 2304: 36 tiles 6.6, few 4.6;
-//   64     64 x 64 tiles: fp32 (bound by its matrix rate, and the smaller tiles fill the chip evenly: 6144 x 768 from 768 72 us, with
+//   few    (forward) fewer than 64 tiles of 64 x 64: there a block a tile leaves most of the chip idle.  200 x 768 from 768 in
+//          bf16: 48 tiles 7.0 us, few 5.1; 14 x 2304: 36 tiles 6.6, few 4.6; but 480 x 768: 96 tiles 6.6, few 9.6;
+//   64     64 x 64 tiles: fp32 (bound by its matrix rate, and the smaller tiles fill the chip evenly: 6144 x 768 from 768 70 us, with
 //          128 x 64 80) and 16-bit products with fewer than 160 tiles of 128 x 128 (1000 x 776 from 776: 7.6 us against 10.2);
 //   128    up to 512 tiles of 256 x 256 (8192 x 1536 from 768: 25 us; 256 x 256 25.6, 64 x 64 31);
 //   256    from there on, forward only: L2 to LDS moves 14.5 TB/s over the chip, which 128 x 128 tiles of 16-bit values need in full
 //          (49152 x 2304 from 768: 184 us against 187; 8192 x 8192 from 8192: 907 us against 1192).
-// A contraction is split over blocks when the output alone would leave compute units idle; each part is at least eight steps long,
-// which pays for writing and joining its fp32 outputs.
+// 16-bit blocks stay and walk over tiles (128 x 128: 212 us against 226 with a block a tile); fp32 ones do not (49152 x 768 from 768:
+// 454 us against 513).
+// A contraction is split over blocks when the output alone would leave compute units idle: for weight gradients, whose contraction is
+// the batch (1536 x 768 from 8192 tokens: 30 us and 9 to join, unsplit 64), for less than 64 tiles (fp32, whose steps take longer, 128:
+// 480 x 768 from 768 17 us, whole 20), and for long contractions on less than 256 (1000 x 768 from 2304: fp32 41 us, whole 53; bf16
+// 18 and 20); each part is at least eight steps long.  Elsewhere joining costs what the shorter parts save (1536 x 1024 from 1024
+// in bf16 in two parts: 20 us, whole 10; 1000 x 776 from 776 in fp32: 26, whole 21).
 enum Kernel { kAny, kFew, k64, k128, k256 };
 struct Plan { Kernel kernel; int parts; int64_t k_split; };
 
@@ -26,12 +31,14 @@ Plan plan_of(int dtype, bool a_t, bool b_t, bool whole, int64_t m, int64_t n, in
   const int64_t step = dtype == 0 ? 32 : 64;
   Plan p{kAny, 1, std::max<int64_t>(k, 1)};
   auto tiles = [&](int64_t s) { return cdiv(m, s) * cdiv(n, s); };
+  const int64_t t128 = std::max<int64_t>(1, tiles(128)), t64 = std::max<int64_t>(1, tiles(64));
   if (whole && k > 0) {
-    if (!a_t && !b_t && tiles(64) < 128) { p.kernel = kFew; return p; }
+    if (!a_t && !b_t && t64 < 64) { p.kernel = kFew; return p; }
     if (!a_t && !b_t && dtype != 0 && tiles(256) >= 512) { p.kernel = k256; return p; }
   }
-  const int64_t t128 = std::max<int64_t>(1, tiles(128)), parts128 = std::min<int64_t>({512 / t128, k / (8 * step), 64});
-  const int64_t t64 = std::max<int64_t>(1, tiles(64)), parts64 = std::min<int64_t>({1024 / t64, k / (8 * step), 64});
+  const bool may_split = a_t || t64 < (dtype == 0 ? 128 : 64) || (k >= 2048 && t64 < 256);
+  const int64_t parts128 = may_split ? std::min<int64_t>({512 / t128, k / (8 * step), 64}) : 1;
+  const int64_t parts64 = may_split ? std::min<int64_t>({1024 / t64, k / (8 * step), 64}) : 1;
   int64_t parts;
   if (whole && k > 0) {
     p.kernel = dtype != 0 && t128 * std::max<int64_t>(1, parts128) >= 160 ? k128 : k64;
@@ -65,10 +72,12 @@ hipError_t launch_with(const GemmArgs& a, GemmParams p, const Plan& plan) {
         else gemm_few_kernel<T, ACT, 4><<<dim3(cols, (unsigned)cdiv(a.m, 64)), 512, 0, a.st>>>(p);
       }
       return hipGetLastError();
-    case k64:
+    case k64: {
+      const int64_t ti64 = cdiv(a.m, 64) * cdiv(a.n, 64);
       if (split) tile<T, AT, BT, 0, true, 64, 64, 2, 2, 4>(a, p, plan.parts, 0);
-      else tile<T, AT, BT, ACT, false, 64, 64, 2, 2, 4>(a, p, 1, sizeof(T) == 4 ? 1280 : 1024);
+      else tile<T, AT, BT, ACT, false, 64, 64, 2, 2, 4>(a, p, 1, sizeof(T) == 4 ? ti64 : 1024);
       break;
+    }
     case k128:
       if constexpr (sizeof(T) == 2) {
         if (split) tile<T, AT, BT, 0, true, 128, 128, 4, 2, 4>(a, p, plan.parts, 0);

@@ -60,7 +60,7 @@ class MPNetEncoder:
         self._stamp = None
 
     def _frozen(self):
-        stamp = tuple((id(p), p.data_ptr(), p._version) for p in self.model.encoder.parameters())
+        stamp = tuple((id(p), p.data_ptr(), -1 if p.is_inference() else p._version) for p in self.model.encoder.parameters())
         if stamp != self._stamp:
             with torch.no_grad():
                 self._laid_out = self._layers()
