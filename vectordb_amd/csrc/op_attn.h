@@ -505,6 +505,38 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams 
   if (p.lse && lane < 32 && i0 + l < len) p.lse[(long long)head * p.total + s.begin + i0 + l] = any ? m + __log2f(sum) : INFINITY;
 }
 
+// A 32x32 tile's sums by distance, keys in the registers.  Register r's key is row(r) and a lane's query 16 b + c, so shifting the 16
+// lanes of a row by s = row & 15 brings distances row - 16 b - c that are alike but for a multiple of 16 to one lane: what stays
+// inside belongs to 16 (row >> 4) - 16 b - c, what is pushed out and comes in again at the other end to 16 more.  Two shifted
+// additions a register (one instruction each) into three sums; the middle one's halves go to the outer two; and two additions to
+// the half's line in LDS, where a lane meets only its own residue of 32 (tiles begin at multiples of 32), so that plain reads and
+// writes serve.  64 texts of 16 to 384 tokens, 12 heads: the dq kernel without bucket sums takes 49 us, with these 61; with one LDS
+// atomic a score it took 296 (an LDS float atomic of a wave holds the LDS about 190 cycles).
+template <int CTRL> __device__ __forceinline__ float shifted(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));     // 0 where nothing comes in
+}
+template <int R> __device__ __forceinline__ void add_shifted(float (&sum)[3], const f32x16& x) {
+  if constexpr (R < 16) {
+    constexpr int row = (R & 3) + 8 * (R >> 2), k = row >> 4, s = row & 15;
+    if constexpr (s == 0) {
+      sum[k] += x[R];
+    } else {
+      sum[k] += shifted<0x100 + s>(x[R]);              // lane c gets lane c + s
+      sum[k + 1] += shifted<0x110 + 16 - s>(x[R]);     // lane c gets lane c + s - 16
+    }
+    add_shifted<R + 1>(sum, x);
+  }
+}
+__device__ __forceinline__ void add_diagonals(float* mine, int e0, const f32x16& x) {
+  const int l = threadIdx.x & 31;
+  float sum[3] = {};
+  add_shifted<0>(sum, x);
+  const float other = __shfl_xor(sum[1], 16, 64);      // distance 16 - (l ^ 16): -l for l below 16, else 32 - l
+  float* at = mine + e0 - l;
+  at[0] += sum[0] + (l < 16 ? other : 0.f);
+  at[32] += sum[2] + (l < 16 ? 0.f : other);
+}
+
 // part[t] = bucket t's sum of the lines hist [lines][span] by distance and of what lies beyond R (far): the lines joined in order,
 // then eight lanes per bucket.
 __device__ __forceinline__ void fold_buckets(const AttnParams& p, float* hist, const float (*far)[2], int lines, int span, float* part) {
@@ -582,10 +614,8 @@ __device__ __forceinline__ float ds_lift(const AttnParams& p, int head, long lon
 }
 
 // dq and the block's part of dtable: like the forward pass, with ds^T in the place of p^T.
-// The bucket sums: each half of a wave adds its tile's ds by distance into a line of its own in LDS.  The additions are LDS
-// atomics only because lanes meet at an address in DIFFERENT instructions: the 32 lanes of a half hold 32 different distances
-// at every step, and a wave's LDS operations keep their order, so nothing depends on timing.  Tiles beyond R go into two
-// registers.  One thread per bucket then adds up its distances, in order.
+// The bucket sums: each half of a wave adds its tile's ds by distance into a line of its own in LDS; tiles beyond R go into two
+// registers.  One block's lines are folded into buckets in a fixed order, and the blocks' buckets by attention_dtable_kernel.
 template <typename T, int DP, int NW, bool DTABLE>
 __global__ __launch_bounds__(NW * 64) void attention_dq_any_kernel(const AttnParams p) {
   constexpr int V = Elem<T>::kVec, BQ = NW * 32;
@@ -649,11 +679,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_any_kernel(const AttnPar
         for (int r = 0; r < 16; ++r) x += t[r];
         if (e0 > 0) above += x; else below += x;
       } else {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int e = e0 + (r & 3) + 8 * (r >> 2) + 4 * half - (lane & 31);
-          __hip_atomic_fetch_add(mine + e, t[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
-        }
+        add_diagonals(mine + 4 * half, e0, t);
       }
     }
     if (lift != 1.f) t *= lift;
@@ -731,26 +757,6 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_any_kernel(const AttnPa
 }
 
 // ---- backward, whole 16-byte pieces and head widths of 32, 64 and 128 -------------------------------------------------------
-// A 32x32 tile's sums by distance, keys in the registers: every register's 32 lanes of a half are turned by their row number, which
-// brings equal distances to one lane; what wraps round goes to a second sum.  Sixteen lane moves and two additions to the
-// half's line in LDS; adding each score to the line by LDS atomics instead cost 250 us of a 428 us pass (64 texts of 16 to 384
-// tokens, 12 heads).
-__device__ __forceinline__ void add_diagonals(float* mine, int e0, const f32x16& x) {
-  const int lane = threadIdx.x & 63, l = lane & 31;
-  float a = 0.f, b = 0.f;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int row = (r & 3) + 8 * (r >> 2);
-    const float v = __int_as_float(__builtin_amdgcn_ds_bpermute(((lane & 32) | ((l + row) & 31)) << 2, __float_as_int(x[r])));
-    const bool in = l + row < 32;          // the value's column is l + row: distance -l, or beyond the edge 32 - l
-    a += in ? v : 0.f;
-    b += in ? 0.f : v;
-  }
-  // 32 distances each, no two lanes of a half alike; a wave's LDS operations keep their order
-  __hip_atomic_fetch_add(mine + e0 - l, a, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
-  __hip_atomic_fetch_add(mine + e0 - l + 32, b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
-}
-
 // dq and the block's bucket sums.  Each wave: 32 queries, one per lane column; key tiles of 64 through LDS.  k is read along its rows (scores) and across them (ds k): one copy in LDS, in the order of the transposed reads, serves
 // both - the reads along it meet two by two on a bank.
 template <typename T, int D, int NW, bool DTABLE>
