@@ -106,6 +106,9 @@ def test_hip_engine_sees_changed_weights(tmp_path, hip_lib):
         fresh = MPNetEmbedder(d, device="cuda:0", engine="hip", autocast=amp)
         fresh.model.load_state_dict(hip.model.state_dict())
         assert torch.equal(fresh.embed_device(TEXTS), after)
+        fresh.model.encoder.layer[0].output.dense.bias.data.add_(1.0)       # a write that leaves no trace: only once asked
+        fresh.refresh()
+        assert not torch.equal(fresh.embed_device(TEXTS), after)
 
 
 @pytest.mark.gpu

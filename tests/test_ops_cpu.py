@@ -114,6 +114,14 @@ def test_pool_refusals(hip_lib):
     _refused(hip_lib, rc, "NULL")
 
 
+def test_no_gpu_means_loud_failure(hip_lib):
+    if torch.cuda.is_available():
+        pytest.skip("a GPU is present")
+    assert hip_lib.vdb_op_linear_dev(0, 1, P, 8, P, 8, None, None, 0, P, 8, None, 4, 8, 8, 0, None, 0, None) == -2
+    assert hip_lib.vdb_op_mean_pool_dev(0, 0, P, 8, P, 2, 10, 8, 1, P, None, None) == -2
+    assert b"mean_pool" in hip_lib.vdb_last_error(None)
+
+
 def test_python_refuses_what_is_not_on_a_gpu():
     x, w = torch.zeros(3, 4), torch.zeros(5, 4)
     with pytest.raises(ValueError, match="GPU"):

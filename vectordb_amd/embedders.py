@@ -90,6 +90,11 @@ class MPNetEmbedder:
         tokens = self.tok(list(texts), padding=False, truncation=True, max_length=self.max_length)["input_ids"] if len(texts) else []
         return self._hip.encode(*self._hip.pack(tokens, self.device))
 
+    def refresh(self) -> None:
+        """engine="hip": lay the weights out again, after writes through `parameter.data` (other changes are seen)."""
+        if self._hip is not None:
+            self._hip.refresh()
+
     def embed_device(self, texts: Sequence[str]):
         """-> torch.Tensor [n, dim] fp32 on self.device, rows unit length.  On a GPU the result can go
         straight into the store (Collection.add accepts it; vdb_add_dev) without the host round trip

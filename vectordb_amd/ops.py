@@ -13,7 +13,9 @@ zeros, and so do their gradients).  The offsets are read on the device: a captur
 
 float32, bfloat16 and float16, one type per call; sums, softmax and norms are 32-bit.  Everything runs on the current stream of
 the tensors' GPU, scratch comes from torch's allocator, nothing waits for the GPU, and results do not depend on timing.  There
-is no CPU fallback: tensors elsewhere raise ValueError.  torch.autocast does not reach in here: cast first."""
+is no CPU fallback: tensors elsewhere raise ValueError.  torch.autocast does not reach in here: cast first.  Calls can be captured
+into HIP graphs; for a captured backward pass, take leaves of their own inside the capture (t.detach().requires_grad_()) and
+torch.autograd.grad, as with any torch function: leaves that an eager graph holds as well accumulate on another stream."""
 from __future__ import annotations
 
 import functools
