@@ -321,10 +321,11 @@ __device__ __forceinline__ void add_across(f32x16 (&acc)[D / 32], const T* s, in
 
 // line[kMargin + R + e] = bias(e) / scale, |e| <= R + kMargin: the start value of a tile's sums, so that a tile near the diagonal costs a
 // look-up a score and no arithmetic.  Finite values stay within what the later product with scale log2(e) can hold: a row
-// of the type's lowest value has a softmax.
+// of the type's lowest value has a softmax.  Only the distances that a text of this length meets are filled in (around: its length and
+// a tile; a far tile, which takes its bias from an end of the line, is met only where all of it is).
 constexpr int kMargin = 64;
 template <typename T>
-__device__ __forceinline__ void make_start_line(float* line, const AttnParams& p, int head, float c) {
+__device__ __forceinline__ void make_start_line(float* line, const AttnParams& p, int head, float c, int around) {
   __shared__ float tab[128];
   const float most = 3e38f / fmaxf(c, 1.f);
   for (int t = threadIdx.x; t < p.n_buckets; t += blockDim.x) {
@@ -332,7 +333,8 @@ __device__ __forceinline__ void make_start_line(float* line, const AttnParams& p
     tab[t] = __builtin_isinf(b) ? b : fminf(fmaxf(b / p.scale, -most), most);
   }
   __syncthreads();
-  for (int t = threadIdx.x; t <= 2 * (p.reach + kMargin); t += blockDim.x) line[t] = tab[bucket_of(p.bk, t - p.reach - kMargin)];
+  const int middle = p.reach + kMargin, w = around < middle ? around : middle;
+  for (int t = middle - w + threadIdx.x; t <= middle + w; t += blockDim.x) line[t] = tab[bucket_of(p.bk, t - middle)];
 }
 
 // Waits for what the compiler has loaded into x, here: left to itself it waits where x is used first, inside the loop over tiles, and
@@ -405,13 +407,13 @@ template <typename T> __device__ __forceinline__ void add_pair(float& sum, float
   else sum += a + b;
 }
 
-// Block: one slot of NW * 32 queries of one head, 32 queries a wave, one per lane column; key tiles of 64 (fp32: 32, which lets
-// more blocks share a compute unit: 576 blocks of 16 x 384 tokens, 12 heads, would take two turns of 512), the next one under way
+// Block: one slot of NW * 32 queries of one head, 32 queries a wave, one per lane column; key tiles of 64 (fp32 and
+// blocks of two waves: 32, which lets more blocks share a compute unit: 512 texts of 3 to 64 tokens 24.7 -> 20.8 us), the next one under way
 // while one is multiplied.  Per score: one product-and-add, one exponential, half a maximum, one sum, half a conversion; the
 // running sums are rescaled only when a maximum has moved.
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams p, unsigned slots, unsigned hop) {
-  constexpr int BQ = NW * 32, KT = sizeof(T) == 4 ? 32 : 64, V = Elem<T>::kVec;
+  constexpr int BQ = NW * 32, KT = sizeof(T) == 4 || NW == 2 ? 32 : 64, V = Elem<T>::kVec;
   using KR = Rows<T, D, kRow>;
   using VR = Rows<T, D, kCol>;
   __shared__ __align__(1024) T buf[2][2][KT * D];          // [turn][k, v]
@@ -445,7 +447,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams 
     for (int x = 0; x < D / (2 * V); ++x) fq[x] = *(const typename Elem<T>::vec*)(q + x * 2 * V);
   }
   const float c = p.scale * kLog2e;
-  make_start_line<T>(line, p, head, c);
+  make_start_line<T>(line, p, head, c, len + KT);
   const float* mid = line + p.reach + kMargin + 4 * half - l;      // mid[e0 + row] = start value of row (+ 4 half), column l
 #pragma unroll
   for (int x = 0; x < D / (2 * V); ++x) settle(fq[x]);
@@ -821,7 +823,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
   const float lift = ds_lift<T>(p, head, s.b);
   const float c = p.scale * kLog2e;
   float* hist = line + span + 1;
-  make_start_line<T>(line, p, head, c);
+  make_start_line<T>(line, p, head, c, len + KT);
   if constexpr (DTABLE) for (int t = threadIdx.x; t < NW * 2 * span; t += NW * 64) hist[t] = 0.f;
   const float* mid = line + reach + kMargin + 4 * half - l;
   float* mine = hist + (wave * 2 + half) * span + reach + kMargin + 4 * half;       // mine[e0 + row - column]
@@ -930,7 +932,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
   }
   const float lift = ds_lift<T>(p, head, s.b);
   const float c = p.scale * kLog2e;
-  make_start_line<T>(line, p, head, c);
+  make_start_line<T>(line, p, head, c, len + QT);
   const float* mid = line + p.reach + kMargin - 4 * half + l;        // mid[e0 - row]: column l is the key, the rows are queries
 #pragma unroll
   for (int x = 0; x < D / (2 * V); ++x) { settle(fk[x]); settle(fv[x]); }
