@@ -945,7 +945,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
     if (j0 >= len) continue;
     const T* sq = buf[t & 1][0];
     const T* sg = buf[t & 1][1];
-#pragma unroll
+#pragma unroll 1
     for (int u = 0; u < QT / 32; ++u) {
       if (t * QT + u * 32 >= len) break;
       const int e0 = j0 - t * QT - u * 32;
