@@ -114,6 +114,22 @@ def test_linear_gradients_large(ops, dtype, m, n, k, name):
     assert all(torch.equal(p, q) for p, q in zip(grads, again))
 
 
+@pytest.mark.parametrize("m,n,k,name", [(1999, 636, 644, "gelu"), (1537, 1024, 1020, "relu"), (6100, 768, 72, "none")])
+def test_linear_tiles_that_spread_evenly(ops, m, n, k, name):
+    """fp32 products whose 64 x 64 tiles leave some compute units one more than others: the tiles of 96 rows, with ragged edges."""
+    g = torch.Generator(device="cuda").manual_seed(m + n + k)
+    x, w, b, r, dy = (torch.randn(*s, generator=g, device="cuda") for s in ((m, k), (n, k), (n,), (m, n), (m, n)))
+    w = w * k ** -0.5
+    if name == "relu":      # keep the sums off the step
+        z = x.double() @ w.double().t() + b.double()
+        dy = torch.where(z.abs() < 1e-4, torch.zeros_like(dy), dy)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = ops.linear(x, w, b, name, r)
+    grads = torch.autograd.grad(y, leaves, dy)
+    with torch.no_grad():
+        hold([y, *grads], ref.linear(x, w, b, name, r, dy))
+
+
 def test_linear_layouts_strides_and_alignment(ops):
     g = torch.Generator().manual_seed(5)
     for dtype in TYPES:

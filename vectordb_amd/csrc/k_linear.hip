@@ -12,8 +12,11 @@ int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 //   any    a row or a width that is no whole number of 16-byte pieces;
 //   few    (forward) fewer than 64 tiles of 64 x 64: there a block a tile leaves most of the chip idle.  200 x 768 from 768 in
 //          bf16: 48 tiles 7.0 us, few 5.1; 14 x 2304: 36 tiles 6.6, few 4.6; but 480 x 768: 96 tiles 6.6, few 9.6;
-//   64     64 x 64 tiles: fp32 (bound by its matrix rate, and the smaller tiles fill the chip evenly: 6144 x 768 from 768 70 us, with
-//          128 x 64 80) and 16-bit products with fewer than 160 tiles of 128 x 128 (1000 x 776 from 776: 7.6 us against 10.2);
+//   64     64 x 64 tiles: fp32, bound by its matrix rate, where the smaller tiles fill the chip evenly (next line), and 16-bit
+//          products with fewer than 160 tiles of 128 x 128 (1000 x 776 from 776: 7.6 us against 10.2);
+//   96     fp32, 96 x 64 tiles where they spread more evenly: the time goes by the fullest compute unit.  64 x 64 gives some units
+//          five tiles where the mean is 4.5, 96 x 64 gives each three: 6144 x 768 from 768 61 us, 64 x 64 69, 128 x 64 80;
+//          6144 x 768 from 2048 149 and 172; 1536 x 1024 from 1024 34 and 40; 1999 x 640 from 640 24 and 28;
 //   128    up to 512 tiles of 256 x 256 (8192 x 1536 from 768: 25 us; 256 x 256 25.6, 64 x 64 31);
 //   256    from there on, forward only: L2 to LDS moves 14.5 TB/s over the chip, which 128 x 128 tiles of 16-bit values need in full
 //          (49152 x 2304 from 768: 184 us against 187; 8192 x 8192 from 8192: 907 us against 1192).
@@ -24,7 +27,7 @@ int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // 480 x 768 from 768 17 us, whole 20), and for long contractions on less than 256 (1000 x 768 from 2304: fp32 41 us, whole 53; bf16
 // 18 and 20); each part is at least eight steps long.  Elsewhere joining costs what the shorter parts save (1536 x 1024 from 1024
 // in bf16 in two parts: 20 us, whole 10; 1000 x 776 from 776 in fp32: 26, whole 21).
-enum Kernel { kAny, kFew, k64, k128, k256 };
+enum Kernel { kAny, kFew, k64, k96, k128, k256 };
 struct Plan { Kernel kernel; int parts; int64_t k_split; };
 
 Plan plan_of(int dtype, bool a_t, bool b_t, bool whole, int64_t m, int64_t n, int64_t k) {
@@ -43,6 +46,7 @@ Plan plan_of(int dtype, bool a_t, bool b_t, bool whole, int64_t m, int64_t n, in
   if (whole && k > 0) {
     p.kernel = dtype != 0 && t128 * std::max<int64_t>(1, parts128) >= 160 ? k128 : k64;
     parts = p.kernel == k128 ? (t128 >= 256 ? 1 : parts128) : (t64 >= 512 ? 1 : parts64);
+    if (dtype == 0 && !a_t && parts <= 1 && cdiv(cdiv(m, 96) * cdiv(n, 64), 256) * 96 < cdiv(t64, 256) * 64) p.kernel = k96;
   } else {
     parts = t128 >= 128 ? 1 : parts128;
   }
@@ -78,6 +82,9 @@ hipError_t launch_with(const GemmArgs& a, GemmParams p, const Plan& plan) {
       else tile<T, AT, BT, ACT, false, 64, 64, 2, 2, 4>(a, p, 1, sizeof(T) == 4 ? ti64 : 1024);
       break;
     }
+    case k96:
+      if constexpr (sizeof(T) == 4 && !AT) tile<T, AT, BT, ACT, false, 96, 64, 2, 2, 4>(a, p, 1, cdiv(a.m, 96) * cdiv(a.n, 64));
+      break;
     case k128:
       if constexpr (sizeof(T) == 2) {
         if (split) tile<T, AT, BT, 0, true, 128, 128, 4, 2, 4>(a, p, plan.parts, 0);

@@ -149,6 +149,7 @@ template <typename T, bool ACROSS, int ROWS, int THREADS>
 struct TileOperand {
   static constexpr int V = Elem<T>::kVec, KB = 8 * V, kPieces = ROWS * 8 / THREADS;   // pieces of 16 bytes per thread and step
   static constexpr int kChunksRow = ACROSS ? ROWS / V : 8;                           // 16-byte pieces per LDS row
+  static_assert(ROWS * 8 % THREADS == 0 && THREADS % 128 == 0 && (!ACROSS || (ROWS & (ROWS - 1)) == 0), "whole pieces; the XOR stays inside a row");
   static __device__ __forceinline__ int swizzle(int row) {
     if constexpr (!ACROSS) return (row >> 1) & 7;
     else if constexpr (sizeof(T) == 4) return ((row >> 2) & 3) << 2;
