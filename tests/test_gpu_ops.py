@@ -227,6 +227,22 @@ def test_attention_forward_and_gradients(ops, dtype, name, heads, d):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [32, 64, 128, 96])
+@pytest.mark.parametrize("lengths", [[63], [64], [65, 62], [127, 0, 64], [383], [384], [700, 389]], ids=str)
+def test_attention_average_lengths(ops, dtype, d, lengths):
+    """Both sides of the average lengths at which the width of a block changes."""
+    t, heads = DT[dtype], 2
+    g = torch.Generator().manual_seed(sum(lengths) + d)
+    total = sum(lengths)
+    qkv, table, dout = rnd(g, total, 3, heads, d, dtype=t), rnd(g, 32, heads, dtype=t), rnd(g, total, heads, d, dtype=t)
+    off = offsets_of(lengths)
+    want = ref.attention(qkv, table, off.tolist(), d ** -0.5, 128, dout)
+    lq, lt = qkv.cuda().requires_grad_(), table.cuda().requires_grad_()
+    out = ops.bucketed_attention(lq, lt, off)
+    hold([out, *torch.autograd.grad(out, [lq, lt], dout.cuda())], want, f"{lengths} {dtype}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n_buckets,max_distance", [(4, 2), (4, 512), (6, 9), (32, 128), (32, 9), (32, 512), (64, 100), (128, 33), (128, 512)])
 def test_attention_buckets(ops, dtype, n_buckets, max_distance):
     t = DT[dtype]

@@ -7,11 +7,13 @@ namespace {
 
 // Waves per block (32 queries or keys each), by the average length, which is all the host knows: a block that is wider than its
 // sequence leaves waves idle, one that is narrower loads the sequence's rows, and looks up its place and its bias, more often.
-// 512 texts of 3 to 64 tokens, 12 heads of 32, fp16: two waves 26 us, four 32; 1000 texts of 10 to 70, heads of 64, bf16: 94 and 80;
-// 384 tokens each: 73 and 59.  One wave was slower everywhere.
-int tile_waves(int64_t n_seqs, int64_t total) {
+// Two waves and four, us, 12 heads.  Forward, bf16, heads of 64: 600 texts of 10 to 70 tokens 37 and 51, 64 each 43 and 49, 64 x 384
+// 62 and 59, 4095 + 2564 + 1033 174 and 125; fp32, 600 of 40 to 104 232 and 226.  With the backward pass, bf16, heads of 64: 10 to 70
+// 215 and 236, 64 each 326 and 296.  Only the 16-bit backward pass of heads of 128, whose tiles fill the LDS with two blocks, gains
+// from more of them for longer: 100 x 256 521 and 622, 384 857 and 922, 500 to 1000 3213 and 2985.  One wave was slower everywhere.
+int tile_waves(int dtype, int d, bool back, int64_t n_seqs, int64_t total) {
   const int64_t mean = n_seqs ? total / n_seqs : 0;
-  return mean < 40 ? 2 : 4;
+  return mean < (back && dtype != 0 && d > 64 ? 384 : 64) ? 2 : 4;
 }
 
 AttnParams params(const AttnArgs& a, int elem) {
@@ -80,7 +82,7 @@ hipError_t backward(const AttnParams& p, const AttnArgs& a) {
 
 template <typename T, int DP>
 hipError_t run_dp(const AttnParams& p, const AttnArgs& a, bool back) {
-  switch (tile_waves(p.n_seqs, p.total)) {
+  switch (tile_waves(sizeof(T) == 4 ? 0 : 1, p.d, back, p.n_seqs, p.total)) {
     case 2: return back ? backward<T, DP, 2>(p, a) : forward<T, DP, 2>(p, a.st);
     default: return back ? backward<T, DP, 4>(p, a) : forward<T, DP, 4>(p, a.st);
   }
@@ -106,10 +108,6 @@ hipError_t run_t(const AttnArgs& a, bool back) {
 }
 
 int64_t pad256(int64_t x) { return (x + 255) / 256 * 256; }
-int64_t part_bytes(int64_t n_seqs, int64_t total, int heads, int n_buckets) {
-  return pad256(n_slots(total, n_seqs, 32 * tile_waves(n_seqs, total)) * heads * n_buckets * 4);
-}
-
 }  // namespace
 
 hipError_t launch_attention(int dtype, const AttnArgs& a) {
@@ -117,8 +115,8 @@ hipError_t launch_attention(int dtype, const AttnArgs& a) {
 }
 
 int64_t attention_backward_workspace(int dtype, int64_t n_seqs, int64_t total, int heads, int d, int n_buckets) {
-  (void)d;
-  return pad256(total * heads * 4) + (dtype == 2 ? pad256(2 * n_seqs * heads * 4) : 0) + part_bytes(n_seqs, total, heads, n_buckets);
+  const int64_t slots = n_slots(total, n_seqs, 32 * tile_waves(dtype, d, true, n_seqs, total));
+  return pad256(total * heads * 4) + (dtype == 2 ? pad256(2 * n_seqs * heads * 4) : 0) + pad256(slots * heads * n_buckets * 4);
 }
 
 hipError_t launch_attention_backward(int dtype, AttnArgs a, char* ws) {
