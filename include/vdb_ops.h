@@ -15,6 +15,7 @@
  * calls that may overlap need two); nothing is allocated, no call waits for the device, and every launch can be captured
  * into a HIP graph.  All pointers are device memory on `device`, the stream is one of that device's; the calling
  * thread's current device is left as it was.  Element strides (ld*) are in elements; the last dimension is contiguous.
+ * Limits: m up to 2^29; n, k and dim up to 2^20; (total / 32 + n_seqs + 1) times the heads below 2^24.
  * Results do not depend on the order in which blocks run: there is no floating-point atomic between two of them.
  */
 #ifndef VDB_OPS_H

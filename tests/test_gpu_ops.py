@@ -587,6 +587,20 @@ def test_other_streams_and_two_calls_at_once(ops):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_forward_mode_derivatives_are_refused(ops):
+    """A tangent is never dropped without a word."""
+    from torch.autograd import forward_ad
+    x, w, off = torch.ones(5, 8, device="cuda"), torch.ones(4, 8, device="cuda"), offsets_of([2, 3])
+    q, table = torch.ones(5, 3, 1, 8, device="cuda"), torch.ones(32, 1, device="cuda")
+    with forward_ad.dual_level():
+        for call in (lambda: ops.linear(forward_ad.make_dual(x, x), w), lambda: ops.linear(x, forward_ad.make_dual(w, w), activation="gelu"),
+                     lambda: ops.bucketed_attention(forward_ad.make_dual(q, q), table, off), lambda: ops.mean_pool(forward_ad.make_dual(x, x), off)):
+            with pytest.raises(NotImplementedError):
+                call()
+        assert torch.equal(ops.linear(x, w), torch.full((5, 4), 8.0, device="cuda"))
+    assert torch.equal(ops.linear(x, w), torch.full((5, 4), 8.0, device="cuda"))
+
+
 def test_captured_and_replayed(ops):
     """A whole layer and the pooling in one HIP graph, replayed with other rows and other offsets in between eager calls."""
     g = torch.Generator().manual_seed(10)

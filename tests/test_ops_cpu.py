@@ -114,6 +114,21 @@ def test_pool_refusals(hip_lib):
     _refused(hip_lib, rc, "NULL")
 
 
+def test_sizes_beyond_one_launch_are_refused(hip_lib):
+    """A launch has fewer than 2^32 threads along a dimension: what would need more is refused before it, not by it."""
+    _refused(hip_lib, hip_lib.vdb_op_linear_dev(0, 1, P, 1, P, 1, None, None, 0, P, 1, None, 2 ** 30, 1, 1, 0, None, 0, None), "m must be")
+    _refused(hip_lib, hip_lib.vdb_op_mean_pool_dev(0, 0, P, 8, P, 2 ** 24, 10, 8, 1, P, None, None), "n_seqs")
+    _refused(hip_lib, hip_lib.vdb_op_mean_pool_backward_dev(0, 0, P, P, P, P, 2 ** 23, 2 ** 28, 8, 1, P, None), "n_seqs")
+    _refused(hip_lib, hip_lib.vdb_op_attention_dev(0, 1, P, P, P, 96, 16, P, 32, 128, P, 2 ** 23, 10, 2, 16, 0.25, P, None, None, None), "too many")
+
+
+def test_a_library_without_the_operators_loads(tmp_path):
+    """VECTORDB_AMD_LIB may name an older build: the store's symbols are what it needs."""
+    import ctypes
+    bare = ctypes.CDLL(None)
+    assert not hasattr(bare, _capi.OP_SYMBOLS[0]) and _capi._declare_ops(bare) is bare
+
+
 def test_no_gpu_means_loud_failure(hip_lib):
     if torch.cuda.is_available():
         pytest.skip("a GPU is present")

@@ -99,6 +99,8 @@ def _declare(lib: C.CDLL) -> C.CDLL:
 
 
 def _declare_ops(lib: C.CDLL) -> C.CDLL:
+    if not hasattr(lib, OP_SYMBOLS[0]):      # a build of before them (VECTORDB_AMD_LIB): the store runs, an operator's call raises
+        return lib
     vp, i32, i64, f32 = C.c_void_p, C.c_int, C.c_int64, C.c_float
     lib.vdb_op_linear_workspace_bytes.argtypes = [i32, i64, i64, i64]
     lib.vdb_op_linear_dev.argtypes = [i32, i32, vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, i64, i64, i64, i32, vp, i64, vp]

@@ -60,7 +60,7 @@ Plan plan_of(int dtype, bool a_t, bool b_t, bool whole, int64_t m, int64_t n, in
 template <typename T, bool AT, bool BT, int ACT, bool SPLIT, int BM, int BN, int WGI, int WGJ, int MINW>
 void tile(const GemmArgs& a, const GemmParams& p, int parts, int64_t resident) {
   const int64_t ti = cdiv(a.m, BM), tj = cdiv(a.n, BN);
-  const dim3 grid((unsigned)(SPLIT ? ti * tj : std::min(ti * tj, resident)), (unsigned)parts);
+  const dim3 grid((unsigned)(SPLIT ? ti * tj : std::min({ti * tj, resident, (int64_t)1 << 22})), (unsigned)parts);
   gemm_tile_kernel<T, AT, BT, ACT, SPLIT, BM, BN, WGI, WGJ, MINW><<<grid, WGI * WGJ * 64, 0, a.st>>>(p, (int)ti, (int)tj);
 }
 

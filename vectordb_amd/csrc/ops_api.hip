@@ -9,7 +9,8 @@ using namespace vdbk;
 
 namespace {
 
-constexpr int64_t kMaxRows = (int64_t)1 << 30, kMaxWidth = (int64_t)1 << 20;
+// a launch has fewer than 2^32 threads along a dimension: 2^24 blocks of 256
+constexpr int64_t kMaxRows = (int64_t)1 << 29, kMaxWidth = (int64_t)1 << 20, kMaxBlocks = ((int64_t)1 << 24) - 1;
 
 int bad(int code, const char* what) {
   set_last_error(what);
@@ -85,13 +86,13 @@ Buckets make_buckets(int n_buckets, int max_distance) {
 int check_attention(int dtype, const void* q, const void* k, const void* v, int64_t ld_t, int64_t ld_h, const void* table, int n_buckets,
                     int max_distance, const int64_t* offsets, int64_t n_seqs, int64_t total, int heads, int d, float scale) {
   NEED(known(dtype), "attention: dtype must be VDB_OP_F32, VDB_OP_BF16 or VDB_OP_F16");
-  NEED(n_seqs >= 0 && n_seqs <= kMaxRows && total >= 0 && total <= kMaxRows, "attention: n_seqs and total must be in [0, 2^30]");
+  NEED(n_seqs >= 0 && n_seqs <= kMaxRows && total >= 0 && total <= kMaxRows, "attention: n_seqs and total must be in [0, 2^29]");
   NEED(heads >= 1 && heads <= 1024, "attention: heads must be in [1, 1024]");
   NEED(d >= 1 && d <= VDB_OP_MAX_HEAD_DIM, "attention: head_dim must be in [1, 128]");
   NEED(n_buckets >= 4 && n_buckets <= VDB_OP_MAX_BUCKETS && n_buckets % 2 == 0, "attention: n_buckets must be even and in [4, 128]");
   NEED(max_distance > n_buckets / 4 && max_distance <= VDB_OP_MAX_DISTANCE, "attention: max_distance must be in (n_buckets / 4, 512]");
   NEED(std::isfinite(scale) && scale > 0.f, "attention: scale must be positive and finite");
-  NEED((total / 32 + n_seqs + 1) * heads < ((int64_t)1 << 31), "attention: too many sequences, rows and heads for one launch");
+  NEED((total / 32 + n_seqs + 1) * heads <= kMaxBlocks, "attention: too many sequences, rows and heads for one launch");
   NEED(total == 0 || (q && k && v && table && offsets), "attention: a pointer is NULL");
   NEED(total == 0 || (ld_t >= 0 && ld_h >= 0), "attention: strides must not be negative");
   return VDB_OK;
@@ -110,7 +111,7 @@ int vdb_op_linear_dev(int device, int dtype, const void* x, int64_t ldx, const v
                       int64_t ldr, void* y, int64_t ldy, void* z, int64_t m, int64_t n, int64_t k, int act, void* workspace,
                       int64_t workspace_bytes, void* stream) {
   NEED(known(dtype), "linear: dtype must be VDB_OP_F32, VDB_OP_BF16 or VDB_OP_F16");
-  NEED(widths(m, n, k), "linear: m must be in [0, 2^30], n and k in [1, 2^20]");
+  NEED(widths(m, n, k), "linear: m must be in [0, 2^29], n and k in [1, 2^20]");
   NEED(act >= VDB_ACT_NONE && act <= VDB_ACT_RELU, "linear: unknown activation");
   if (m == 0) return VDB_OK;
   NEED(x && w && y, "linear: a pointer is NULL");
@@ -144,7 +145,7 @@ int vdb_op_linear_backward_dev(int device, int dtype, const void* dy, int64_t ld
                                const void* z, void* dx, void* dw, void* db, int64_t m, int64_t n, int64_t k, int act, void* workspace,
                                int64_t workspace_bytes, void* stream) {
   NEED(known(dtype), "linear_backward: dtype must be VDB_OP_F32, VDB_OP_BF16 or VDB_OP_F16");
-  NEED(widths(m, n, k), "linear_backward: m must be in [0, 2^30], n and k in [1, 2^20]");
+  NEED(widths(m, n, k), "linear_backward: m must be in [0, 2^29], n and k in [1, 2^20]");
   NEED(act >= VDB_ACT_NONE && act <= VDB_ACT_RELU, "linear_backward: unknown activation");
   NEED(m == 0 || dy, "linear_backward: dy is NULL");
   NEED(m == 0 || ((!dw || x) && (!dx || w)), "linear_backward: x is needed for dw, w for dx");
@@ -219,8 +220,8 @@ int vdb_op_attention_backward_dev(int device, int dtype, const void* q, const vo
 int vdb_op_mean_pool_dev(int device, int dtype, const void* hidden, int64_t ld, const int64_t* offsets, int64_t n_seqs, int64_t total,
                          int64_t dim, int normalize, float* y, float* inv_norm, void* stream) {
   NEED(known(dtype), "mean_pool: dtype must be VDB_OP_F32, VDB_OP_BF16 or VDB_OP_F16");
-  NEED(n_seqs >= 0 && n_seqs <= kMaxRows && total >= 0 && total <= kMaxRows && dim >= 1 && dim <= kMaxWidth,
-       "mean_pool: n_seqs and total must be in [0, 2^30], dim in [1, 2^20]");
+  NEED(n_seqs >= 0 && n_seqs <= kMaxBlocks && total >= 0 && total <= kMaxRows && dim >= 1 && dim <= kMaxWidth,
+       "mean_pool: n_seqs must be in [0, 2^24), total in [0, 2^29], dim in [1, 2^20]");
   if (n_seqs == 0) return VDB_OK;
   NEED(offsets && y && (hidden || total == 0), "mean_pool: a pointer is NULL");
   NEED(ld >= dim, "mean_pool: the row stride is smaller than a row");
@@ -233,8 +234,8 @@ int vdb_op_mean_pool_dev(int device, int dtype, const void* hidden, int64_t ld, 
 int vdb_op_mean_pool_backward_dev(int device, int dtype, const float* dy, const float* y, const float* inv_norm, const int64_t* offsets,
                                   int64_t n_seqs, int64_t total, int64_t dim, int normalize, void* dhidden, void* stream) {
   NEED(known(dtype), "mean_pool_backward: dtype must be VDB_OP_F32, VDB_OP_BF16 or VDB_OP_F16");
-  NEED(n_seqs >= 0 && n_seqs <= kMaxRows && total >= 0 && total <= kMaxRows && dim >= 1 && dim <= kMaxWidth,
-       "mean_pool_backward: n_seqs and total must be in [0, 2^30], dim in [1, 2^20]");
+  NEED(n_seqs >= 0 && total >= 0 && total <= kMaxRows && n_seqs <= kMaxBlocks - 1 - total / 32 && dim >= 1 && dim <= kMaxWidth,
+       "mean_pool_backward: n_seqs + total / 32 must be below 2^24, dim in [1, 2^20]");
   if (total == 0) return VDB_OK;
   NEED(offsets && dhidden && (n_seqs == 0 || (dy && y && (inv_norm || !normalize))), "mean_pool_backward: a pointer is NULL");
   ON_DEVICE("mean_pool_backward");

@@ -22,6 +22,7 @@ import functools
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _capi
@@ -108,6 +109,8 @@ def _ld(t: torch.Tensor) -> int:
 
 
 def _wants_grad(*tensors) -> bool:
+    if getattr(forward_ad, "_current_level", -1) >= 0:      # dual numbers: the autograd function refuses them, a plain call would drop them
+        return True
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
