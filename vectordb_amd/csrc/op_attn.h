@@ -407,9 +407,9 @@ template <typename T> __device__ __forceinline__ void add_pair(float& sum, float
   else sum += a + b;
 }
 
-// Block: one slot of NW * 32 queries of one head, 32 queries a wave, one per lane column; key tiles of 64 (fp32 and
-// blocks of two waves: 32, which lets more blocks share a compute unit: 512 texts of 3 to 64 tokens 24.7 -> 20.8 us), the next one under way
-// while one is multiplied.  Per score: one product-and-add, one exponential, half a maximum, one sum, half a conversion; the
+// Block: one slot of NW * 32 queries of one head, 32 queries a wave, one per lane column; key tiles of 64 (fp32 and blocks of two
+// waves: 32, which lets more blocks share a compute unit: 512 texts of 3 to 64 tokens 20 us, with 64 keys 25), the next one under
+// way while one is multiplied.  Per score: one product-and-add, one exponential, half a maximum, one sum, half a conversion; the
 // running sums are rescaled only when a maximum has moved.
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams p, unsigned slots, unsigned hop) {
@@ -512,7 +512,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams 
 // inside belongs to 16 (row >> 4) - 16 b - c, what is pushed out and comes in again at the other end to 16 more.  Two shifted
 // additions a register (one instruction each) into three sums; the middle one's halves go to the outer two; and two additions to
 // the half's line in LDS, where a lane meets only its own residue of 32 (tiles begin at multiples of 32), so that plain reads and
-// writes serve.  64 texts of 16 to 384 tokens, 12 heads: the dq kernel without bucket sums takes 49 us, with these 61; with one LDS
+// writes serve.  64 texts of 16 to 384 tokens, 12 heads: the dq kernel without bucket sums takes 49 us, with these 59; with one LDS
 // atomic a score it took 296 (an LDS float atomic of a wave holds the LDS about 190 cycles).
 template <int CTRL> __device__ __forceinline__ float shifted(float x) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));     // 0 where nothing comes in
@@ -565,8 +565,9 @@ __device__ __forceinline__ void fold_buckets(const AttnParams& p, float* hist, c
 }
 
 // ---- backward -------------------------------------------------------------------------------------------------------------
-// delta[h][t] = sum_d dout (out + rest) (the general kernels'; attention_dq_kernel has its own); fp16 also the largest |dout| and |v| of each sequence and head (bits of non-negative
-// floats order like integers, so the atomic maximum does not depend on the order of arrival).
+// delta[h][t] = sum_d dout (out + rest) (the general kernels'; attention_dq_kernel has its own); fp16 also the largest |dout| and |v|
+// of each sequence and head (bits of non-negative floats order like integers, so the atomic maximum does not depend on the order
+// of arrival).
 template <typename T, bool PEAK>
 __global__ __launch_bounds__(256) void attention_delta_kernel(const AttnParams p, unsigned* peak) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -759,8 +760,10 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_any_kernel(const AttnPa
 }
 
 // ---- backward, whole 16-byte pieces and head widths of 32, 64 and 128 -------------------------------------------------------
-// dq and the block's bucket sums.  Each wave: 32 queries, one per lane column; key tiles of 64 through LDS.  k is read along its rows (scores) and across them (ds k): one copy in LDS, in the order of the transposed reads, serves
-// both - the reads along it meet two by two on a bank.
+// dq and the block's bucket sums.  Each wave: 32 queries, one per lane column; key tiles of 64 through LDS.  k is read along its
+// rows (scores) and across them (ds k): one copy in LDS, in the order of the transposed reads, serves both - the reads along it
+// meet two by two on a bank.  64 texts of 16 to 384 tokens, 12 heads of 64, bf16: 59 us, 0.26 PFLOP/s, 19 vector instructions a
+// score and 1.8 waves a SIMD on average: their issue and the latency of a chain a tile, about half each.
 template <typename T, int D, int NW, bool DTABLE>
 __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel(const AttnParams p, unsigned slots, unsigned hop) {
   constexpr int BQ = NW * 32, KT = 64, V = Elem<T>::kVec;
@@ -883,7 +886,8 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
 }
 
 // dk and dv: each wave 32 keys, one per lane column; query tiles of 64 through LDS, q and dout once, in the order of the
-// transposed reads.
+// transposed reads.  The two halves of a tile one after the other: held together they cost registers, 63 us instead of 58
+// (0.35 PFLOP/s) at the size above.
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kernel(const AttnParams p, unsigned slots, unsigned hop) {
   constexpr int BQ = NW * 32, QT = 64, V = Elem<T>::kVec;
