@@ -242,6 +242,55 @@ def test_attention_average_lengths(ops, dtype, d, lengths):
     hold([out, *torch.autograd.grad(out, [lq, lt], dout.cuda())], want, f"{lengths} {dtype}")
 
 
+BATCHES = {
+    "mixed": ([200, 0, 1, 384, 64, 65, 127, 128, 129, 300, 33, 0, 90, 90, 17, 250, 5, 160] * 2, 77),
+    "alike": ([128] * 20, 0),
+    "most that are ordered": ([64 + (i * 37) % 9 for i in range(255)] + [0], 3),
+    "one more": ([64 + (i * 37) % 9 for i in range(257)], 0),
+}
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("name", list(BATCHES))
+def test_attention_gradients_of_many_blocks(ops, dtype, d, name):
+    """Batches large enough that the backward pass takes the longest texts first."""
+    lengths, spare = BATCHES[name]
+    t, heads = DT[dtype], 18 if len(lengths) < 100 else 3
+    g = torch.Generator(device="cuda").manual_seed(len(lengths) + d)
+    total = sum(lengths) + spare
+    qkv, dout = (torch.randn(total, *s, heads, d, generator=g, device="cuda").to(t) for s in ((3,), ()))
+    table = torch.randn(32, heads, generator=g, device="cuda").to(t)
+    qkv[total - spare:] = math.nan
+    dout[total - spare:] = math.nan
+    off = offsets_of(lengths)
+    lq, lt = qkv.requires_grad_(), table.requires_grad_()
+    out = ops.bucketed_attention(lq, lt, off)
+    grads = torch.autograd.grad(out, [lq, lt], dout, retain_graph=True)
+    with torch.no_grad():
+        want = ref.attention(qkv.cpu(), table.cpu(), off.tolist(), d ** -0.5, 128, dout.cpu())
+    hold([out, *grads], want, f"{name} {dtype}")
+    again = torch.autograd.grad(out, [lq, lt], dout)
+    assert all(torch.equal(a, b) for a, b in zip(grads, again))
+
+
+def test_attention_order_with_offsets_of_any_content(ops):
+    """Lists that are no offsets at all, at a size where the longest text goes first: nothing leaves its buffers, and the next call is right."""
+    heads, d, n, total = 18, 32, 40, 5000
+    g = torch.Generator(device="cuda").manual_seed(2)
+    qkv = torch.randn(total, 3, heads, d, generator=g, device="cuda").bfloat16().requires_grad_()
+    table = torch.randn(32, heads, generator=g, device="cuda").bfloat16().requires_grad_()
+    dout = torch.randn(total, heads, d, generator=g, device="cuda").bfloat16()
+    good = offsets_of([total // n] * n)
+    want = torch.autograd.grad(ops.bucketed_attention(qkv, table, good), [qkv, table], dout)
+    for off in ([0, total] * (n // 2) + [total], list(range(n + 1))[::-1], [-2 ** 62] * (n + 1), [2 ** 62] * (n + 1), [0] * (n + 1),
+                [0] + [total] * n, [total - 1] * n + [3]):
+        bad = torch.tensor(off, dtype=torch.int64, device="cuda")
+        torch.autograd.grad(ops.bucketed_attention(qkv, table, bad), [qkv, table], dout)
+        got = torch.autograd.grad(ops.bucketed_attention(qkv, table, good), [qkv, table], dout)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n_buckets,max_distance", [(4, 2), (4, 512), (6, 9), (32, 128), (32, 9), (32, 512), (64, 100), (128, 33), (128, 512)])
 def test_attention_buckets(ops, dtype, n_buckets, max_distance):

@@ -23,6 +23,7 @@ struct AttnParams {
   void* out; void* rest; float* lse;
   const void* dout; void *dq, *dk, *dv; long long gld_t, gld_h;
   float* delta; const unsigned* peak; float* part;   // peak: [2][heads][n_seqs] largest |dout| and |v| (fp16 only)
+  const i32x4* order;   // the tiled backward kernels' places, longest sequences first, or nullptr
   int vec;        // q, k, v, out, dout, gradients: 16-byte rows
   int reach;      // R
   Buckets bk;
@@ -760,6 +761,64 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_any_kernel(const AttnPa
 }
 
 // ---- backward, whole 16-byte pieces and head widths of 32, 64 and 128 -------------------------------------------------------
+// The places of the tiled backward kernels, longest sequences first: [slots] of (begin, end, sequence, tile), then the rows behind the
+// last sequence, then nothing (-1).  A block's time goes by its sequence's length, and blocks that begin in the sequences' own order
+// leave the chip waiting for the long ones that began last: 64 texts of 16 to 384 tokens, 12 heads of 64, bf16: 121 us for the
+// backward pass, 111 with this; fp32 516 and 409.  One block; a sequence's place is the tiles of all that come ahead of it, counted
+// by 4 to 16 threads.
+constexpr int kMaxOrdered = 256;
+__global__ __launch_bounds__(1024) static void attention_order_kernel(const int64_t* __restrict__ offsets, int n_seqs, long long total, int tile,
+                                                                      int slots, i32x4* __restrict__ order) {
+  __shared__ int begin[kMaxOrdered], first[kMaxOrdered], used;
+  __shared__ int2 size[kMaxOrdered];                   // rows and tiles
+  const int b = threadIdx.x;
+  if (b == 0) used = 0;
+  if (b < n_seqs) {
+    const int r0 = (int)seq_edge(offsets, b, total), r1 = (int)seq_edge(offsets, b + 1, total), len = r1 > r0 ? r1 - r0 : 0;
+    begin[b] = r0;
+    size[b] = make_int2(len, (len + tile - 1) / tile);
+  }
+  const int end = (int)seq_edge(offsets, n_seqs, total);
+  __syncthreads();
+  const int share = n_seqs <= 64 ? 4 : n_seqs <= 128 ? 3 : 2;      // log2 of the threads that count for one sequence
+  const int mine = threadIdx.x >> share;
+  if (mine < n_seqs) {
+    const int2 me = size[mine];
+    int at = 0;
+#pragma unroll 4
+    for (int o = threadIdx.x & ((1 << share) - 1); o < n_seqs; o += 1 << share) {
+      const int2 x = size[o];
+      at += x.x > me.x || (x.x == me.x && o < mine) ? x.y : 0;
+    }
+    for (int k = 1; k < 1 << share; k <<= 1) at += __shfl_xor(at, k, 64);
+    first[mine] = at;
+    if ((threadIdx.x & ((1 << share) - 1)) == 0) atomicMax(&used, at + me.y);
+  }
+  __syncthreads();
+  // unordered offsets can ask for more places than there are: the bounds hold whatever they say
+  for (int s = threadIdx.x >> 4; s < n_seqs; s += 64)
+    for (int t = threadIdx.x & 15; t < size[s].y && first[s] + t < slots; t += 16) order[first[s] + t] = i32x4{begin[s], begin[s] + size[s].x, s, t};
+  for (int at = used + threadIdx.x; at < slots; at += 1024) {
+    const int t = at - used;
+    order[at] = (long long)t * tile < total - end ? i32x4{end, (int)total, n_seqs, t} : i32x4{0, 0, -1, 0};
+  }
+}
+
+// A block's head and place
+__device__ __forceinline__ Slot place_of(const AttnParams& p, unsigned slots, unsigned hop, int tile, int& head, unsigned& slot) {
+  if (p.order) {
+    slot = blockIdx.x / p.heads;
+    head = blockIdx.x % p.heads;
+    const i32x4 o = p.order[slot];
+    return Slot{__builtin_amdgcn_readfirstlane(o[0]), __builtin_amdgcn_readfirstlane(o[1]), __builtin_amdgcn_readfirstlane(o[2]),
+                __builtin_amdgcn_readfirstlane(o[3])};
+  }
+  const unsigned at = xcd_run(slots * p.heads, hop);
+  head = at / slots;
+  slot = at % slots;
+  return find_slot(p.offsets, p.n_seqs, p.total, tile, slot);
+}
+
 // dq and the block's bucket sums.  Each wave: 32 queries, one per lane column; key tiles of 64 through LDS.  k is read along its
 // rows (scores) and across them (ds k): one copy in LDS, in the order of the transposed reads, serves both - the reads along it
 // meet two by two on a bank.  64 texts of 16 to 384 tokens, 12 heads of 64, bf16: 59 us, 0.26 PFLOP/s, 19 vector instructions a
@@ -773,10 +832,9 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
   __shared__ float far[NW][2];
   extern __shared__ float line[];                          // 2 (R + margin) + 1, then NW * 2 lines of 2 (R + margin)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l = lane & 31;
-  const unsigned at = xcd_run(slots * p.heads, hop);
-  const int head = at / slots;
-  const unsigned slot = at % slots;
-  const Slot s = find_slot(p.offsets, p.n_seqs, p.total, BQ, slot);
+  int head;
+  unsigned slot;
+  const Slot s = place_of(p, slots, hop, BQ, head, slot);
   float* part = p.part + ((long long)slot * p.heads + head) * p.n_buckets;
   if (s.b < 0 || s.b == p.n_seqs) {
     if (s.b >= 0) {
@@ -897,9 +955,9 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
   __shared__ __align__(16) float stat[2][2][QT];             // [turn][lse, delta]
   extern __shared__ float line[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l = lane & 31;
-  const unsigned at = xcd_run(slots * p.heads, hop);
-  const int head = at / slots;
-  const Slot s = find_slot(p.offsets, p.n_seqs, p.total, BQ, at % slots);
+  int head;
+  unsigned slot;
+  const Slot s = place_of(p, slots, hop, BQ, head, slot);
   if (s.b < 0) return;
   if (s.b == p.n_seqs) {
     const long long r0 = s.begin + (long long)s.tile * BQ, r1 = r0 + BQ < s.end ? r0 + BQ : s.end;
