@@ -513,7 +513,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams 
 // inside belongs to 16 (row >> 4) - 16 b - c, what is pushed out and comes in again at the other end to 16 more.  Two shifted
 // additions a register (one instruction each) into three sums; the middle one's halves go to the outer two; and two additions to
 // the half's line in LDS, where a lane meets only its own residue of 32 (tiles begin at multiples of 32), so that plain reads and
-// writes serve.  64 texts of 16 to 384 tokens, 12 heads: the dq kernel without bucket sums takes 49 us, with these 59; with one LDS
+// writes serve.  64 texts of 16 to 384 tokens, 12 heads: the dq kernel without bucket sums took 49 us, with these 59; with one LDS
 // atomic a score it took 296 (an LDS float atomic of a wave holds the LDS about 190 cycles).
 template <int CTRL> __device__ __forceinline__ float shifted(float x) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));     // 0 where nothing comes in
@@ -821,8 +821,8 @@ __device__ __forceinline__ Slot place_of(const AttnParams& p, unsigned slots, un
 
 // dq and the block's bucket sums.  Each wave: 32 queries, one per lane column; key tiles of 64 through LDS.  k is read along its
 // rows (scores) and across them (ds k): one copy in LDS, in the order of the transposed reads, serves both - the reads along it
-// meet two by two on a bank.  64 texts of 16 to 384 tokens, 12 heads of 64, bf16: 59 us, 0.26 PFLOP/s, 19 vector instructions a
-// score and 1.8 waves a SIMD on average: their issue and the latency of a chain a tile, about half each.
+// meet two by two on a bank.  64 texts of 16 to 384 tokens, 12 heads of 64, bf16: 51 us, 0.30 PFLOP/s, 19 vector instructions a
+// score: bound by their issue and by the latency of a chain a tile.
 template <typename T, int D, int NW, bool DTABLE>
 __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel(const AttnParams p, unsigned slots, unsigned hop) {
   constexpr int BQ = NW * 32, KT = 64, V = Elem<T>::kVec;
@@ -944,8 +944,8 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
 }
 
 // dk and dv: each wave 32 keys, one per lane column; query tiles of 64 through LDS, q and dout once, in the order of the
-// transposed reads.  The two halves of a tile one after the other: held together they cost registers, 63 us instead of 58
-// (0.35 PFLOP/s) at the size above.
+// transposed reads.  The two halves of a tile one after the other: held together they cost registers, 63 us
+// instead of 58 at the size above, 52 with the longest texts first (0.39 PFLOP/s).
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kernel(const AttnParams p, unsigned slots, unsigned hop) {
   constexpr int BQ = NW * 32, QT = 64, V = Elem<T>::kVec;
