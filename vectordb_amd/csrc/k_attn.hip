@@ -41,7 +41,7 @@ template <typename T, int DP, int NW>
 hipError_t forward(const AttnParams& p, hipStream_t st) {
   const unsigned slots = (unsigned)n_slots(p.total, p.n_seqs, NW * 32), grid = slots * p.heads;
   if (p.vec && p.d == DP) {
-    attention_kernel<T, DP, NW><<<grid, NW * 64, (2 * (p.reach + kMargin) + 1) * sizeof(float), st>>>(p, slots, hop_of(grid));
+    attention_kernel<T, DP, NW><<<grid, NW * 64, start_span(p.reach) * sizeof(float), st>>>(p, slots, hop_of(grid));
     return hipGetLastError();
   }
   attention_any_kernel<T, DP, NW><<<grid, NW * 64, (2 * p.reach + 1) * sizeof(float), st>>>(p);
@@ -64,12 +64,12 @@ template <typename T, int DP, int NW>
 hipError_t backward(const AttnParams& p, const AttnArgs& a) {
   const int64_t slots = n_slots(p.total, p.n_seqs, NW * 32);
   const unsigned grid = (unsigned)(slots * p.heads);
-  const size_t line = (2 * p.reach + 1) * sizeof(float), hist = (size_t)NW * 2 * 2 * (p.reach + 64) * sizeof(float);
+  const size_t line = (2 * p.reach + 1) * sizeof(float), hist = (size_t)NW * 2 * sums_span(p.reach) * sizeof(float);
   hipError_t e;
   bool done = false;
   if constexpr (sizeof(T) * DP < 512) {
     if (tiled<T>(p)) {
-      const size_t start = (2 * (p.reach + kMargin) + 1) * sizeof(float);
+      const size_t start = start_span(p.reach) * sizeof(float);
       if (p.order) {
         attention_order_kernel<<<1, 1024, 0, a.st>>>(p.offsets, (int)p.n_seqs, p.total, NW * 32, (int)slots, (i32x4*)a.order);
         if ((e = hipGetLastError()) != hipSuccess) return e;

@@ -10,6 +10,7 @@
 // Every product is arranged so that its C registers are the next product's operand (op_common.h): the forward pass and dq
 // compute s^T with the keys in the registers and one query per lane, dk / dv compute s with the queries in the registers.
 #pragma once
+#include "attn_lines.h"
 #include "op_common.h"
 #include "ops.h"
 
@@ -177,7 +178,7 @@ __device__ __forceinline__ void zero_rows(T* base, long long ld, long long first
 template <bool KEYS_IN_ROWS>
 __device__ __forceinline__ void add_bias(f32x16& s, float c, const float* line, int reach, int e0) {
   const int lane = threadIdx.x & 63;
-  if (e0 - 31 >= reach || e0 + 31 <= -reach) {
+  if (tile_is_far(e0, reach)) {
     const float b = line[e0 > 0 ? 2 * reach : 0];
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = s[r] * c + b;
@@ -320,11 +321,10 @@ __device__ __forceinline__ void add_across(f32x16 (&acc)[D / 32], const T* s, in
   }
 }
 
-// line[kMargin + R + e] = bias(e) / scale, |e| <= R + kMargin: the start value of a tile's sums, so that a tile near the diagonal costs a
+// line[start_at(R, e)] = bias(e) / scale, |e| <= R + kMargin: the start value of a tile's sums, so that a tile near the diagonal costs a
 // look-up a score and no arithmetic.  Finite values stay within what the later product with scale log2(e) can hold: a row
 // of the type's lowest value has a softmax.  Only the distances that a text of this length meets are filled in (around: its length and
 // a tile; a far tile, which takes its bias from an end of the line, is met only where all of it is).
-constexpr int kMargin = 64;
 template <typename T>
 __device__ __forceinline__ void make_start_line(float* line, const AttnParams& p, int head, float c, int around) {
   __shared__ float tab[128];
@@ -334,7 +334,7 @@ __device__ __forceinline__ void make_start_line(float* line, const AttnParams& p
     tab[t] = __builtin_isinf(b) ? b : fminf(fmaxf(b / p.scale, -most), most);
   }
   __syncthreads();
-  const int middle = p.reach + kMargin, w = around < middle ? around : middle;
+  const int middle = start_zero(p.reach), w = around < middle ? around : middle;
   for (int t = middle - w + threadIdx.x; t <= middle + w; t += blockDim.x) line[t] = tab[bucket_of(p.bk, t - middle)];
 }
 
@@ -358,9 +358,9 @@ __device__ __forceinline__ float scores(f32x16& x, const T* s, int r0, const typ
                                         const float* line, const float* start) {
   constexpr int N = D / (2 * Elem<T>::kVec);
   float shift = 0.f;
-  const bool is_far = e0 - 31 >= p.reach || e0 + 31 <= -p.reach;
+  const bool is_far = tile_is_far(e0, p.reach);
   if (__builtin_amdgcn_readfirstlane(is_far)) {
-    shift = line[e0 > 0 ? 2 * (p.reach + kMargin) : 0];
+    shift = line[e0 > 0 ? start_span(p.reach) - 1 : 0];
     f32x16 none = {};
     Elem<T>::mma(ROWS::along(s, r0, 0), f[0], none);
     x = none;
@@ -449,7 +449,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams 
   }
   const float c = p.scale * kLog2e;
   make_start_line<T>(line, p, head, c, len + KT);
-  const float* mid = line + p.reach + kMargin + 4 * half - l;      // mid[e0 + row] = start value of row (+ 4 half), column l
+  const float* mid = line + start_at(p.reach, 4 * half - l);      // mid[e0 + row] = start value of row (+ 4 half), column l
 #pragma unroll
   for (int x = 0; x < D / (2 * V); ++x) settle(fq[x]);
   float m = -INFINITY, sum = 0.f;
@@ -530,12 +530,12 @@ template <int R> __device__ __forceinline__ void add_shifted(float (&sum)[3], co
     add_shifted<R + 1>(sum, x);
   }
 }
-__device__ __forceinline__ void add_diagonals(float* mine, int e0, const f32x16& x) {
-  const int l = threadIdx.x & 31;
+__device__ __forceinline__ void add_diagonals(float* mine, int reach, int e0, const f32x16& x) {
+  const int l = threadIdx.x & 31, half = (threadIdx.x & 63) >> 5;
   float sum[3] = {};
   add_shifted<0>(sum, x);
   const float other = __shfl_xor(sum[1], 16, 64);      // distance 16 - (l ^ 16): -l for l below 16, else 32 - l
-  float* at = mine + e0 - l;
+  float* at = mine + sums_at(reach, e0, half, l);
   at[0] += sum[0] + (l < 16 ? other : 0.f);
   at[32] += sum[2] + (l < 16 ? 0.f : other);
 }
@@ -550,14 +550,14 @@ __device__ __forceinline__ void fold_buckets(const AttnParams& p, float* hist, c
     hist[t] = x;
   }
   __syncthreads();
-  const int sub = threadIdx.x & 7;
+  const int sub = threadIdx.x & 7, zero = sums_zero(p.reach);
   for (int t = threadIdx.x >> 3; t < ((p.n_buckets + 7) & ~7); t += blockDim.x >> 3) {
     float x = 0.f;
     if (t < p.n_buckets) {
       const int low = t % p.bk.half, side = t / p.bk.half;
       const int n0 = low <= p.bk.near ? low : p.bk.step[low - p.bk.near - 1];
-      const int n1 = low + 1 == p.bk.half ? span / 2 : low + 1 <= p.bk.near ? low + 1 : p.bk.step[low - p.bk.near];
-      for (int n = (side && n0 == 0 ? 1 : n0) + sub; n < n1; n += 8) x += hist[span / 2 + (side ? n : -n)];
+      const int n1 = low + 1 == p.bk.half ? zero : low + 1 <= p.bk.near ? low + 1 : p.bk.step[low - p.bk.near];
+      for (int n = (side && n0 == 0 ? 1 : n0) + sub; n < n1; n += 8) x += hist[zero + (side ? n : -n)];
       if (sub == 0 && low + 1 == p.bk.half) for (int w = 0; w < lines / 2; ++w) x += far[w][side];
     }
     for (int k = 1; k < 8; k <<= 1) x += __shfl_xor(x, k, 64);
@@ -627,7 +627,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_any_kernel(const AttnPar
   __shared__ __align__(16) T skt[DP * (32 + V)];
   __shared__ __align__(16) T sv[32 * (DP + V)];
   __shared__ float far[NW][2];
-  extern __shared__ float line[];                      // 2R + 1, then NW * 2 lines of 2 (R + 64)
+  extern __shared__ float line[];                      // 2R + 1, then NW * 2 lines of sums
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int head = blockIdx.x % p.heads;
   const long long slot = blockIdx.x / p.heads;
@@ -643,11 +643,11 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_any_kernel(const AttnPar
   }
   const int len = (int)(s.end - s.begin);
   const int i0 = s.tile * BQ + wave * 32, i = i0 + (lane & 31);
-  const int reach = p.reach, span = 2 * (reach + 64);
+  const int reach = p.reach, span = sums_span(reach);
   float* hist = line + 2 * reach + 1;
   make_line<T>(line, p, head);
   if constexpr (DTABLE) for (int t = threadIdx.x; t < NW * 2 * span; t += NW * 64) hist[t] = 0.f;
-  float* mine = hist + (wave * 2 + half) * span + reach + 64;   // mine[e]
+  float* mine = hist + (wave * 2 + half) * span;
   const T* kb = (const T*)p.k + s.begin * p.ld_t + head * p.ld_h;
   const T* vb = (const T*)p.v + s.begin * p.ld_t + head * p.ld_h;
   const long long hd = (long long)p.heads * p.d;
@@ -677,13 +677,13 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_any_kernel(const AttnPar
       t[r] = w == 0.f ? 0.f : w * (dp[r] - delta);
     }
     if constexpr (DTABLE) {
-      if (e0 - 31 >= reach || e0 + 31 <= -reach) {
+      if (tile_is_far(e0, reach)) {
         float x = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) x += t[r];
         if (e0 > 0) above += x; else below += x;
       } else {
-        add_diagonals(mine + 4 * half, e0, t);
+        add_diagonals(mine, reach, e0, t);
       }
     }
     if (lift != 1.f) t *= lift;
@@ -830,7 +830,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
   using RV = Rows<T, D, kRow>;
   __shared__ __align__(1024) T buf[2][2][KT * D];          // [turn][k, v]
   __shared__ float far[NW][2];
-  extern __shared__ float line[];                          // 2 (R + margin) + 1, then NW * 2 lines of 2 (R + margin)
+  extern __shared__ float line[];                          // start values, then NW * 2 lines of sums
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l = lane & 31;
   int head;
   unsigned slot;
@@ -846,7 +846,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
   }
   const int len = (int)(s.end - s.begin), tiles = (len + KT - 1) / KT;
   const int i0 = s.tile * BQ + wave * 32;
-  const int reach = p.reach, span = 2 * (reach + kMargin);
+  const int reach = p.reach, span = sums_span(reach);
   const T* kb = (const T*)p.k + s.begin * p.ld_t + head * p.ld_h;
   const T* vb = (const T*)p.v + s.begin * p.ld_t + head * p.ld_h;
   auto issue = [&](int t) {
@@ -883,11 +883,11 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
   }
   const float lift = ds_lift<T>(p, head, s.b);
   const float c = p.scale * kLog2e;
-  float* hist = line + span + 1;
+  float* hist = line + start_span(reach);
   make_start_line<T>(line, p, head, c, len + KT);
   if constexpr (DTABLE) for (int t = threadIdx.x; t < NW * 2 * span; t += NW * 64) hist[t] = 0.f;
-  const float* mid = line + reach + kMargin + 4 * half - l;
-  float* mine = hist + (wave * 2 + half) * span + reach + kMargin + 4 * half;       // mine[e0 + row - column]
+  const float* mid = line + start_at(reach, 4 * half - l);
+  float* mine = hist + (wave * 2 + half) * span;
 #pragma unroll
   for (int x = 0; x < D / (2 * V); ++x) { settle(fq[x]); settle(fg[x]); }
   float from = -lse, less = delta;
@@ -906,7 +906,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
     for (int u = 0; u < KT / 32; ++u) {
       const int j0 = t * KT + u * 32, e0 = j0 - i0;
       if (j0 >= len) break;
-      const bool is_far = e0 - 31 >= reach || e0 + 31 <= -reach;
+      const bool is_far = tile_is_far(e0, reach);
       f32x16 x, dp = {};
       const float shift = from + c * scores<T, D, R, 1>(x, sk, u * 32, fq, e0, p, line, mid + e0);
 #pragma unroll
@@ -927,7 +927,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
           for (int r = 0; r < 16; ++r) y += x[r];
           if (e0 > 0) above += y; else below += y;
         } else {
-          add_diagonals(mine, e0, x);
+          add_diagonals(mine, reach, e0, x);
         }
       }
       if (lift != 1.f) x *= lift;
@@ -995,7 +995,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
   const float lift = ds_lift<T>(p, head, s.b);
   const float c = p.scale * kLog2e;
   make_start_line<T>(line, p, head, c, len + QT);
-  const float* mid = line + p.reach + kMargin - 4 * half + l;        // mid[e0 - row]: column l is the key, the rows are queries
+  const float* mid = line + start_at(p.reach, l - 4 * half);        // mid[e0 - row]: column l is the key, the rows are queries
 #pragma unroll
   for (int x = 0; x < D / (2 * V); ++x) { settle(fk[x]); settle(fv[x]); }
   f32x16 ak[D / 32] = {}, av[D / 32] = {};
