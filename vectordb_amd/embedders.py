@@ -87,13 +87,15 @@ class MPNetEmbedder:
         enabled (engine="hip"): what fine-tuning on matched products steps through.  All texts as one batch; no dropout."""
         if self._hip is None:
             raise ValueError("encode() needs engine='hip'")
+        return self._hip.encode(*self._packed(texts))
+
+    def _packed(self, texts: Sequence[str]):
         tokens = self.tok(list(texts), padding=False, truncation=True, max_length=self.max_length)["input_ids"] if len(texts) else []
-        return self._hip.encode(*self._hip.pack(tokens, self.device))
+        return self._hip.pack(tokens, self.device)
 
     def refresh(self) -> None:
-        """engine="hip": lay the weights out again, after writes through `parameter.data` (other changes are seen)."""
-        if self._hip is not None:
-            self._hip.refresh()
+        """Nothing to do: engine="hip" lays the weights out for every call of encode() and embed_device(), from what the model's
+        parameters hold then.  Here for programs that ask for it after a change."""
 
     def embed_device(self, texts: Sequence[str]):
         """-> torch.Tensor [n, dim] fp32 on self.device, rows unit length.  On a GPU the result can go
@@ -104,9 +106,10 @@ class MPNetEmbedder:
         out = torch.empty((len(texts), self.dim), dtype=torch.float32, device=self.device)
         dev_type = "cuda" if str(self.device).startswith("cuda") else "cpu"
         with torch.no_grad():
+            weights = self._hip.lay_out() if self._hip is not None and texts else None
             for i in range(0, len(texts), self.batch_size):
                 if self._hip is not None:
-                    out[i:i + self.batch_size] = self.encode(texts[i:i + self.batch_size])
+                    out[i:i + self.batch_size] = self._hip.encode(*self._packed(texts[i:i + self.batch_size]), weights)
                     continue
                 enc = self.tok(texts[i:i + self.batch_size], padding=True, truncation=True,
                                max_length=self.max_length, return_tensors="pt").to(self.device)

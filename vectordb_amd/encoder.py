@@ -37,35 +37,64 @@ class MPNetEncoder:
         self.heads = int(cfg.num_attention_heads)
         self.pad = int(cfg.pad_token_id)
         self.max_positions = int(model.embeddings.position_embeddings.weight.shape[0])
-        self._laid_out = None
-        self._stamp = None
 
     # -- weights -------------------------------------------------------------
+    def _modules(self):
+        for layer in self.model.encoder.layer:
+            a = layer.attention.attn
+            yield a, layer.attention.LayerNorm, layer.intermediate.dense, layer.output.dense, layer.output.LayerNorm
+
     def _layers(self):
         """The weights as the operators take them, differentiable."""
-        enc, dt = self.model.encoder, self.dtype
+        dt = self.dtype
         layers = []
-        for layer in enc.layer:
-            a = layer.attention.attn
+        for a, norm, up, down, norm2 in self._modules():
             layers.append((
                 torch.cat([a.q.weight, a.k.weight, a.v.weight]).to(dt), torch.cat([a.q.bias, a.k.bias, a.v.bias]).to(dt),
-                a.o.weight.to(dt), a.o.bias.to(dt), layer.attention.LayerNorm.weight.to(dt), layer.attention.LayerNorm.bias.to(dt),
-                layer.intermediate.dense.weight.to(dt), layer.intermediate.dense.bias.to(dt),
-                layer.output.dense.weight.to(dt), layer.output.dense.bias.to(dt), layer.output.LayerNorm.weight.to(dt), layer.output.LayerNorm.bias.to(dt)))
-        return enc.relative_attention_bias.weight.to(dt), layers
+                a.o.weight.to(dt), a.o.bias.to(dt), norm.weight.to(dt), norm.bias.to(dt), up.weight.to(dt), up.bias.to(dt),
+                down.weight.to(dt), down.bias.to(dt), norm2.weight.to(dt), norm2.bias.to(dt)))
+        return self.model.encoder.relative_attention_bias.weight.to(dt), layers
+
+    def lay_out(self):
+        """The same without gradients: what encode() computes with under no_grad, and takes as its `weights` where a program runs
+        several batches on the same ones.  All copies go into one buffer by one call (12 layers of 768: 0.2 ms of host time in fp32, where
+        only the three projections are joined, 0.27 in 16 bits; 0.38 and 1.13 tensor by tensor).  They are made anew for every call, from
+        what the parameters hold then, on the stream that uses them: nothing tells reliably whether a parameter has changed (fused
+        optimisers and replayed graphs count no version), and copies kept for later would have to be waited for by other streams
+        and outlive the graphs captured with them."""
+        dt = self.dtype
+        sources, places, layers = [], [], []
+        at = 0
+
+        def copied(*parts):
+            """-> (offset, shape) of the parts one behind the other, the first on a 16-byte border."""
+            nonlocal at
+            at = (at + 7) & -8
+            begin = at
+            for p in parts:
+                sources.append(p)
+                places.append(at)
+                at += p.numel()
+            return begin, (sum(p.shape[0] for p in parts), *parts[0].shape[1:])
+
+        def taken(p):
+            return p if p.dtype == dt else copied(p)
+
+        with torch.no_grad():
+            table = taken(self.model.encoder.relative_attention_bias.weight)
+            for a, norm, up, down, norm2 in self._modules():
+                layers.append((copied(a.q.weight, a.k.weight, a.v.weight), copied(a.q.bias, a.k.bias, a.v.bias),
+                               *(taken(p) for m in (a.o, norm, up, down, norm2) for p in (m.weight, m.bias))))
+            flat = torch.empty(at, dtype=dt, device=sources[0].device)
+
+            def view(begin, shape):
+                return flat.as_strided(shape, (shape[1], 1) if len(shape) == 2 else (1,), begin)
+            torch._foreach_copy_([view(b, p.shape) for b, p in zip(places, sources)], sources)
+            return (table if isinstance(table, torch.Tensor) else view(*table),
+                    [tuple(w if isinstance(w, torch.Tensor) else view(*w) for w in layer) for layer in layers])
 
     def refresh(self) -> None:
-        """Lay the weights out again.  encode() does so by itself after an in-place change (an optimiser's step, load_state_dict)
-        or a replaced parameter; only writes through `parameter.data` go unseen."""
-        self._stamp = None
-
-    def _frozen(self):
-        stamp = tuple((id(p), p.data_ptr(), -1 if p.is_inference() else p._version) for p in self.model.encoder.parameters())
-        if stamp != self._stamp:
-            with torch.no_grad():
-                self._laid_out = self._layers()
-            self._stamp = stamp
-        return self._laid_out
+        """Nothing to do: the weights are laid out for every call.  Here for programs that ask for it after a change."""
 
     # -- forward -------------------------------------------------------------
     def pack(self, token_lists: Sequence[Sequence[int]], device) -> tuple:
@@ -85,11 +114,11 @@ class MPNetEncoder:
         flat = torch.tensor(ids + places + ends, dtype=torch.int64).to(device)
         return flat[:n], flat[n:2 * n], flat[2 * n:]
 
-    def encode(self, ids: torch.Tensor, places: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    def encode(self, ids: torch.Tensor, places: torch.Tensor, offsets: torch.Tensor, weights=None) -> torch.Tensor:
         """Packed tokens -> float32 [n_texts, hidden], unit length.  With gradients enabled it is differentiable in the model's
-        parameters."""
+        parameters (unless weights, of lay_out(), are given)."""
         emb = self.model.embeddings
-        table, layers = self._layers() if torch.is_grad_enabled() else self._frozen()
+        table, layers = weights or (self._layers() if torch.is_grad_enabled() else self.lay_out())
         x = emb.word_embeddings(ids) + emb.position_embeddings(places)
         hidden = x.shape[1]
         x = F.layer_norm(x, (hidden,), emb.LayerNorm.weight, emb.LayerNorm.bias, self.eps).to(self.dtype)
