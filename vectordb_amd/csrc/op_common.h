@@ -82,7 +82,7 @@ template <typename T, int ACT> __device__ __forceinline__ float act_slope(float 
   if constexpr (ACT == 1) {
     float bell;
     const float cdf = normal_cdf<T>(z, bell);
-    return cdf + z * 0.3989422804014327f * bell;
+    return cdf + (bell == 0.f ? 0.f : z * 0.3989422804014327f * bell);   // a kept sum of -inf: 0 * inf stays out
   }
   if constexpr (ACT == 2) {
     const float c = 0.79788456080286536f, u = c * (z + 0.044715f * z * z * z);
