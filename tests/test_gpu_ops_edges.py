@@ -40,3 +40,50 @@ def test_activation_gradients_of_sums_beyond_fp16(ops, name):
         assert torch.equal(dx[:, 0].float(), slope * 48 * 300)
         assert torch.equal(dw[:, 0].float(), (slope * xs[:, 0].float()).sum().half().float().expand(48))
         assert torch.equal(db.float(), slope.sum().expand(48))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [24, 32, 64, 128])
+@pytest.mark.parametrize("lengths", [[14], [33, 70, 5], [129, 64, 257], [31] * 40], ids=["one", "ragged", "tiles", "many"])
+def test_attention_infinite_values(ops, dtype, d, lengths):
+    """An infinity in a text's v reaches the column it stands in, as p > 0 times it, and no other; so does one in dout's rows for dv.
+    The last row of a text is where a kernel that repeats it behind the text's end would meet it again."""
+    t, heads = DT[dtype], 2
+    g = torch.Generator().manual_seed(sum(lengths) + d)
+    off = offsets_of(lengths)
+    ends = off.tolist()
+    total = ends[-1]
+    qkv, table, dout = rnd(g, total, 3, heads, d, dtype=t, scale=0.5), rnd(g, 32, heads, dtype=t, scale=0.5), rnd(g, total, heads, d, dtype=t)
+    last = [e - 1 for e in ends[1:]]
+    zero, inf = qkv.clone(), qkv.clone()
+    for x, a, b in ((zero, 0.0, 0.0), (inf, math.inf, -math.inf)):
+        x[last, 2, :, 0], x[last, 2, :, 1] = a, b
+    want, got = (ops.bucketed_attention(x.cuda(), table.cuda(), off).cpu() for x in (zero, inf))
+    assert (got[..., 0] == math.inf).all() and (got[..., 1] == -math.inf).all()
+    assert torch.equal(got[..., 2:], want[..., 2:])
+    gz, gi = dout.clone(), dout.clone()
+    gz[last, :, 0], gi[last, :, 0] = 0.0, math.inf
+    grads = []
+    for do in (gz, gi):
+        leaf = qkv.cuda().requires_grad_()
+        dq, = torch.autograd.grad(ops.bucketed_attention(leaf, table.cuda(), off), [leaf], do.cuda())
+        grads.append(dq[:, 2].cpu())
+    assert (grads[1][..., 0] == math.inf).all()
+    assert torch.equal(grads[1][..., 1:], grads[0][..., 1:])
+
+
+@pytest.mark.parametrize("d", [24, 32, 64, 128])
+def test_attention_probabilities_below_fp16s_normal_range(ops, d):
+    """One key holds nearly all of a row's weight, 4000 others 2^-16 of it each: together 6 %.  In fp16 2^-16 is a subnormal, off by at
+    most 2^-25, 2^-9 of it."""
+    n = 4001
+    qkv = torch.zeros(n, 3, 1, d, dtype=torch.float16)
+    qkv[:, 0, 0, 0] = 8
+    qkv[7, 1, 0, 0] = 16 * math.log(2) / 8 * math.sqrt(d)
+    qkv[:, 2] = 1
+    qkv[7, 2] = 0
+    small = math.exp(-8 * float(qkv[7, 1, 0, 0]) / math.sqrt(d))
+    part = (n - 1) * small / (1 + (n - 1) * small)
+    out = ops.bucketed_attention(qkv.cuda(), torch.zeros(32, 1, dtype=torch.float16, device="cuda"), offsets_of([n])).cpu().double()
+    # the score, of size 11, is off by (d + 6) E 11; the sum's terms by 2^-9; the rounded output by half a step
+    assert ((out - part).abs() <= part * (2.0 ** -9 + 11 * (d + 20) * ref.E + n * ref.E + ref.half_step(torch.float16))).all()

@@ -293,14 +293,24 @@ template <typename T, int D, Order O> struct Rows {
     }
     return x;
   }
-  // N rows from g on to LDS by direct loads; rows past `left` repeat the last one there is
-  template <int N, int THREADS> static __device__ __forceinline__ void load(T* s, const T* g, long long ld, int left) {
+  // N rows from g on to LDS by direct loads.  Rows past `left` repeat the last one there is, or (ZEROS) are zeros, written by the lanes
+  // that would have loaded them: what is multiplied by a p of 0 there may not be an infinity.
+  template <int N, int THREADS, bool ZEROS = false> static __device__ __forceinline__ void load(T* s, const T* g, long long ld, int left) {
     constexpr int kPieces = N * C / THREADS;
     static_assert(N * C % THREADS == 0, "whole turns");
     const unsigned dst = (unsigned)(size_t)(__attribute__((address_space(3))) void*)s + (unsigned)__builtin_amdgcn_readfirstlane((threadIdx.x >> 6) << 10);
+    if (ZEROS && left < N) {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int L = i * THREADS + threadIdx.x, row = L / C;
+        if (row < left) lds_load16(g, (unsigned)(((unsigned)row * (unsigned)ld + (unsigned)(((L % C) ^ swz(row)) * V)) * (unsigned)sizeof(T)), dst + i * (THREADS * 16));
+        else *(i32x4*)((char*)s + L * 16) = i32x4{0, 0, 0, 0};
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
-      const int L = i * THREADS + threadIdx.x, row = L / C, r = row < left ? row : left - 1;
+      const int L = i * THREADS + threadIdx.x, row = L / C, r = ZEROS || row < left ? row : left - 1;
       lds_load16(g, (unsigned)(((unsigned)r * (unsigned)ld + (unsigned)(((L % C) ^ swz(row)) * V)) * (unsigned)sizeof(T)), dst + i * (THREADS * 16));
     }
   }
@@ -437,7 +447,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams 
   auto issue = [&](int t) {
     const int left = len - t * KT;
     KR::template load<KT, NW * 64>(buf[t & 1][0], kb + (long long)t * KT * p.ld_t, p.ld_t, left);
-    VR::template load<KT, NW * 64>(buf[t & 1][1], vb + (long long)t * KT * p.ld_t, p.ld_t, left);
+    VR::template load<KT, NW * 64, true>(buf[t & 1][1], vb + (long long)t * KT * p.ld_t, p.ld_t, left);
   };
   issue(0);
   typename Elem<T>::vec fq[D / (2 * V)];
@@ -976,7 +986,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
   auto issue = [&](int t) {
     const int left = len - t * QT;
     R::template load<QT, NW * 64>(buf[t & 1][0], qb + (long long)t * QT * p.ld_t, p.ld_t, left);
-    R::template load<QT, NW * 64>(buf[t & 1][1], gb + (long long)t * QT * hd, hd, left);
+    R::template load<QT, NW * 64, true>(buf[t & 1][1], gb + (long long)t * QT * hd, hd, left);
     if (threadIdx.x < QT) {
       const bool there = (int)threadIdx.x < left;
       next_lse = there ? lse[t * QT + threadIdx.x] : INFINITY;
