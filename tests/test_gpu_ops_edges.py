@@ -87,3 +87,30 @@ def test_attention_probabilities_below_fp16s_normal_range(ops, d):
     out = ops.bucketed_attention(qkv.cuda(), torch.zeros(32, 1, dtype=torch.float16, device="cuda"), offsets_of([n])).cpu().double()
     # the score, of size 11, is off by (d + 6) E 11; the sum's terms by 2^-9; the rounded output by half a step
     assert ((out - part).abs() <= part * (2.0 ** -9 + 11 * (d + 20) * ref.E + n * ref.E + ref.half_step(torch.float16))).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_mean_pool_keeps_nan(ops, dtype):
+    """A NaN in a text's rows makes its norm NaN: the whole vector, and the whole gradient.  The other texts' do not change."""
+    t = DT[dtype]
+    for dim in (40, 37, 768):
+        g = torch.Generator().manual_seed(dim)
+        for count in (4, 600):                        # both widths of a block
+            off = offsets_of([5, 9, 2, 6] * (count // 4))
+            ends = off.tolist()
+            x, dy = rnd(g, ends[-1], dim, dtype=t), rnd(g, count, dim)
+            bad = x.clone()
+            bad[ends[1] + 3, 11] = math.nan
+            outs = []
+            for h in (x, bad):
+                leaf = h.cuda().requires_grad_()
+                y = ops.mean_pool(leaf, off)
+                dh, = torch.autograd.grad(y, [leaf], dy.cuda())
+                outs.append((y.detach().cpu(), dh.cpu()))
+            (y0, d0), (y1, d1) = outs
+            assert torch.isnan(y1[1]).all() and torch.isnan(d1[ends[1]:ends[2]]).all()
+            keep = [i for i in range(count) if i != 1]
+            rows = [i for i in range(ends[-1]) if not ends[1] <= i < ends[2]]
+            assert torch.equal(y1[keep], y0[keep]) and torch.equal(d1[rows], d0[rows])
+            plain = ops.mean_pool(bad.cuda(), off, normalize=False).cpu()
+            assert torch.isnan(plain[1]).sum() == 1 and torch.isnan(plain).sum() == 1

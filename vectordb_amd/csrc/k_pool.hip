@@ -71,7 +71,7 @@ __global__ __launch_bounds__(THREADS) void mean_pool_kernel(const T* __restrict_
     }
   }
   if (!normalize) return;
-  const float inv = 1.f / fmaxf(sqrtf(block_sum(sq, red)), kTiny);
+  const float norm = sqrtf(block_sum(sq, red)), inv = 1.f / (norm < kTiny ? kTiny : norm);      // NaN stays: the vector's, and the gradient's
   for (int p0 = 0; p0 < pieces; p0 += THREADS) {       // the values that this thread wrote
     const int n = pieces - p0 < THREADS ? pieces - p0 : THREADS, c = p0 + threadIdx.x;
     if ((int)threadIdx.x < n)
