@@ -88,6 +88,27 @@ def test_every_change_of_the_weights_shows(dtype, how):
         first = now
 
 
+@pytest.mark.parametrize("pad", [0, 1, 3])
+def test_positions_count_as_the_models_whatever_its_pad_token(pad):
+    """The model numbers positions by a padding index of its own, not by the configuration's pad token."""
+    model = model_of(pad_token_id=pad)
+    assert float((vectors(encoder_of(model)) - models_own(model)).abs().max()) < 2e-6
+
+
+def test_buckets_are_the_models_whatever_its_table():
+    """The model looks up 32 buckets: the first rows of a larger table, whose others have no gradient.  A smaller one is refused."""
+    model = model_of(relative_attention_num_buckets=64)
+    with torch.no_grad():
+        model.encoder.relative_attention_bias.weight.normal_(generator=torch.Generator().manual_seed(5))
+    enc = encoder_of(model)
+    assert float((vectors(enc) - models_own(model)).abs().max()) < 2e-6
+    vectors(enc, grad=True).sum().backward()
+    grad = model.encoder.relative_attention_bias.weight.grad
+    assert grad[:32].any() and not grad[32:].any()
+    with pytest.raises(ValueError, match="16 buckets"):
+        encoder_of(model_of(relative_attention_num_buckets=16))
+
+
 def test_nothing_is_kept_between_calls():
     """No tensor outlives a call, so no later call on another stream, and no captured graph, can meet one that is unwritten or freed."""
     enc = encoder_of(model_of(), torch.bfloat16)

@@ -16,8 +16,8 @@ from . import ops
 
 #: names of the transformers configuration -> ops.linear's
 _ACTIVATIONS = {"gelu": "gelu", "gelu_new": "gelu_tanh", "gelu_pytorch_tanh": "gelu_tanh", "relu": "relu"}
-#: the model's bucketing ends here whatever its configuration says (its number of buckets is the table's)
-MAX_DISTANCE = 128
+#: the model's bucketing, whatever its configuration says: it uses a larger table's first rows, and fails on a smaller one
+BUCKETS, MAX_DISTANCE = 32, 128
 
 
 class MPNetEncoder:
@@ -30,12 +30,14 @@ class MPNetEncoder:
             raise ValueError(f"hidden_act {cfg.hidden_act!r} is not one of {sorted(_ACTIVATIONS)}")
         if cfg.hidden_size % cfg.num_attention_heads or cfg.hidden_size // cfg.num_attention_heads > 128:
             raise ValueError(f"heads of {cfg.hidden_size}/{cfg.num_attention_heads} values are not supported (whole, at most 128)")
+        if model.encoder.relative_attention_bias.weight.shape[0] < BUCKETS:
+            raise ValueError(f"a position bias of {model.encoder.relative_attention_bias.weight.shape[0]} buckets is not supported (the model looks up {BUCKETS})")
         self.model = model
         self.dtype = dtype
         self.activation = _ACTIVATIONS[cfg.hidden_act]
         self.eps = float(cfg.layer_norm_eps)
         self.heads = int(cfg.num_attention_heads)
-        self.pad = int(cfg.pad_token_id)
+        self.pad = int(model.embeddings.padding_idx)      # positions count from behind it; the model takes 1 whatever cfg.pad_token_id says
         self.max_positions = int(model.embeddings.position_embeddings.weight.shape[0])
 
     # -- weights -------------------------------------------------------------
@@ -43,6 +45,9 @@ class MPNetEncoder:
         for layer in self.model.encoder.layer:
             a = layer.attention.attn
             yield a, layer.attention.LayerNorm, layer.intermediate.dense, layer.output.dense, layer.output.LayerNorm
+
+    def _table(self):
+        return self.model.encoder.relative_attention_bias.weight[:BUCKETS]
 
     def _layers(self):
         """The weights as the operators take them, differentiable."""
@@ -53,7 +58,7 @@ class MPNetEncoder:
                 torch.cat([a.q.weight, a.k.weight, a.v.weight]).to(dt), torch.cat([a.q.bias, a.k.bias, a.v.bias]).to(dt),
                 a.o.weight.to(dt), a.o.bias.to(dt), norm.weight.to(dt), norm.bias.to(dt), up.weight.to(dt), up.bias.to(dt),
                 down.weight.to(dt), down.bias.to(dt), norm2.weight.to(dt), norm2.bias.to(dt)))
-        return self.model.encoder.relative_attention_bias.weight.to(dt), layers
+        return self._table().to(dt), layers
 
     def lay_out(self):
         """The same without gradients: what encode() computes with under no_grad, and takes as its `weights` where a program runs
@@ -81,7 +86,7 @@ class MPNetEncoder:
             return p if p.dtype == dt else copied(p)
 
         with torch.no_grad():
-            table = taken(self.model.encoder.relative_attention_bias.weight)
+            table = taken(self._table())
             for a, norm, up, down, norm2 in self._modules():
                 layers.append((copied(a.q.weight, a.k.weight, a.v.weight), copied(a.q.bias, a.k.bias, a.v.bias),
                                *(taken(p) for m in (a.o, norm, up, down, norm2) for p in (m.weight, m.bias))))
