@@ -88,6 +88,24 @@ def test_every_change_of_the_weights_shows(dtype, how):
         first = now
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_what_runs_between_the_layers_is_32_bits(dtype):
+    """Layers whose products are all 0 leave embeddings, sums and normalisations: nothing there is rounded to 16 bits.  (Four
+    normalisations with gains of order one in 32 bits on both sides; one rounding to 16 bits would be 1e-4 and more.)"""
+    model = model_of()
+    g = torch.Generator().manual_seed(3)
+    with torch.no_grad():
+        for n, p in model.named_parameters():
+            if "LayerNorm" in n:
+                p.normal_(generator=g)
+            elif n.startswith("encoder.layer"):
+                p.zero_()
+    enc = encoder_of(model, dtype)
+    want = models_own(model)
+    assert float((vectors(enc) - want).abs().max()) < 2e-6
+    assert float((vectors(enc, grad=True) - want).abs().max()) < 2e-6
+
+
 @pytest.mark.parametrize("pad", [0, 1, 3])
 def test_positions_count_as_the_models_whatever_its_pad_token(pad):
     """The model numbers positions by a padding index of its own, not by the configuration's pad token."""
