@@ -157,3 +157,23 @@ def test_bucket_rule():
     assert got[:8] == list(range(8)) and got[8] == 8 and got[127] == got[199] == 15 and got == sorted(got)
     assert got.index(10) == 16 and got.index(12) == 32 and got.index(14) == 64      # 8 * 16^(2/8), 16^(4/8), 16^(6/8): whole numbers
     assert [ref.bucket(n, 32, 128) for n in range(1, 200)] == [b + 16 for b in got[1:]]
+
+
+def test_tracers_are_refused():
+    """A trace would hold the outputs' allocation alone and return whatever the memory held."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+    x, w, off = torch.zeros(3, 4), torch.zeros(5, 4), torch.tensor([0, 3])
+    q, table = torch.zeros(3, 3, 2, 8), torch.zeros(32, 2)
+    calls = ((lambda a: ops.linear(a, w), x), (lambda a: ops.bucketed_attention(a, table, off), q), (lambda a: ops.mean_pool(a, off), x))
+    for call, arg in calls:
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(call, (arg,))
+        for kw in (dict(), dict(tracing_mode="fake"), dict(pre_dispatch=True)):
+            with pytest.raises(RuntimeError, match="traced"):
+                make_fx(call, **kw)(arg)
+        for _ in range(2):                       # nothing of it lasts, and a mode that traces nothing refuses nothing (but the CPU is refused)
+            with pytest.raises(ValueError, match="GPU"):
+                call(arg)
+        with FlopCounterMode(display=False), pytest.raises(ValueError, match="GPU"):
+            call(arg)

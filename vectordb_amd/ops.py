@@ -13,7 +13,8 @@ zeros, and so do their gradients).  The offsets are read on the device: a captur
 
 float32, bfloat16 and float16, one type per call; sums, softmax and norms are 32-bit.  Everything runs on the current stream of
 the tensors' GPU, scratch comes from torch's allocator, nothing waits for the GPU, and results do not depend on timing.  There
-is no CPU fallback: tensors elsewhere raise ValueError.  torch.autocast does not reach in here: cast first.  Calls can be captured
+is no CPU fallback: tensors elsewhere raise ValueError.  torch.autocast does not reach in here: cast first.  torch.jit.trace and make_fx
+would record the outputs' allocation alone: under them the calls raise RuntimeError (torch.compile runs them as they are).  Calls can be captured
 into HIP graphs; for a captured backward pass, take leaves of their own inside the capture (t.detach().requires_grad_()) and
 torch.autograd.grad, as with any torch function: leaves that an eager graph holds as well accumulate on another stream."""
 from __future__ import annotations
@@ -66,8 +67,23 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
+_is_tracing, _modes, _key_included = torch._C._is_tracing, torch._C._len_torch_dispatch_stack, torch._C._dispatch_tls_is_dispatch_key_included
+_PRE_DISPATCH = torch._C.DispatchKey.PreDispatch
+
+
+def _refuse_tracing() -> None:
+    """Tracers see torch's own operators only: what a kernel writes would be missing from the trace."""
+    tracing = _is_tracing()
+    if not tracing and (_modes() or _key_included(_PRE_DISPATCH)):
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode
+        tracing = get_proxy_mode() is not None
+    if tracing:
+        raise RuntimeError("vectordb_amd.ops cannot be traced: torch.jit.trace and make_fx would record the output's allocation without the kernel that writes it")
+
+
 def _first(t, name: str) -> int:
     """Check a call's leading tensor; -> the C ABI's number of its type."""
+    _refuse_tracing()
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor; got {type(t).__name__}")
     if not t.is_cuda:
