@@ -7,7 +7,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import ops_reference as ref  # noqa: E402
-from test_gpu_ops import DT, TYPES, offsets_of, rnd  # noqa: E402
+from test_gpu_ops import DT, TYPES, hold, offsets_of, rnd  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -114,3 +114,26 @@ def test_mean_pool_keeps_nan(ops, dtype):
             assert torch.equal(y1[keep], y0[keep]) and torch.equal(d1[rows], d0[rows])
             plain = ops.mean_pool(bad.cuda(), off, normalize=False).cpu()
             assert torch.isnan(plain[1]).sum() == 1 and torch.isnan(plain).sum() == 1
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [24, 32, 64, 128])
+@pytest.mark.parametrize("scale", [2e-38, 1e-30, 1e-18, 1e18, 1e30, 1e38])
+def test_attention_scales_far_from_one(ops, dtype, d, scale):
+    """With q = 0 (or a scale so small that q.k vanishes) the scores are the bias alone, whatever the scale."""
+    t, lengths = DT[dtype], [50, 17]
+    g = torch.Generator().manual_seed(d)
+    qkv, table, dout = rnd(g, 67, 3, 2, d, dtype=t), rnd(g, 32, 2, dtype=t, scale=20.0), rnd(g, 67, 2, d, dtype=t)
+    qkv[:, 0] = 0 if scale > 1 else 0.5
+    qkv[:, 1] *= 0.125
+    off = offsets_of(lengths)
+    want = ref.attention(qkv, table, off.tolist(), scale, 128, dout)
+    lq, lt = qkv.cuda().requires_grad_(), table.cuda().requires_grad_()
+    out = ops.bucketed_attention(lq, lt, off, scale=scale)
+    grads = torch.autograd.grad(out, [lq, lt], dout.cuda())
+    # biases of up to 80 take probabilities below 2^-126, where they are 0: ds is off by 2^-126 |dp - delta| at each of a bucket's places
+    # (at most 50^2 + 17^2 of them), dv by 2^-126 |dout| at each of a key's (at most 50)
+    most = float(dout.abs().max())
+    far_ds, far_dv = 2.0 ** -126 * 2800 * 2 * d * most * float(qkv[:, 2].abs().max()), 2.0 ** -126 * 50 * most
+    hold([out, grads[1]], [want[0], (want[2][0], want[2][1] + far_ds)], f"{scale} {dtype}")
+    hold([grads[0][:, 2]], [(want[1][0][:, 2], want[1][1][:, 2] + far_dv)], f"dv {scale} {dtype}")

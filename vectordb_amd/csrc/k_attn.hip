@@ -37,10 +37,14 @@ unsigned hop_of(unsigned n) {
   return 1;
 }
 
+// The tiled kernels let the bias enter a product that is scaled afterwards, as bias / scale: with a scale far from 1 that quotient leaves
+// the 32-bit range (100 / 1e-37) or its normal part, and the bias would be lost.  The general kernels add it behind the scaling.
+bool even_scale(float s) { return s >= 1e-18f && s <= 1e18f; }
+
 template <typename T, int DP, int NW>
 hipError_t forward(const AttnParams& p, hipStream_t st) {
   const unsigned slots = (unsigned)n_slots(p.total, p.n_seqs, NW * 32), grid = slots * p.heads;
-  if (p.vec && p.d == DP) {
+  if (p.vec && p.d == DP && even_scale(p.scale)) {
     attention_kernel<T, DP, NW><<<grid, NW * 64, start_span(p.reach) * sizeof(float), st>>>(p, slots, hop_of(grid));
     return hipGetLastError();
   }
@@ -50,7 +54,7 @@ hipError_t forward(const AttnParams& p, hipStream_t st) {
 
 // Which backward kernels serve.  fp32 heads of 128 stay with the general ones: two gradients and two operands of 128 words a row
 // are more than the 512 registers of a lane.
-template <typename T> bool tiled(const AttnParams& p) { return p.vec && (p.d == 32 || p.d == 64 || (p.d == 128 && sizeof(T) == 2)); }
+template <typename T> bool tiled(const AttnParams& p) { return p.vec && even_scale(p.scale) && (p.d == 32 || p.d == 64 || (p.d == 128 && sizeof(T) == 2)); }
 
 // Whether the tiled backward kernels take the longest sequences first (attention_order_kernel, one block: the sequences it can count,
 // 3 to 8 us).  Without and with, us, 12 heads of 64, bf16: 64 texts of 16 to 384 tokens 121 and 111, 64 x 384 217 and 194, 32 x 64 to
