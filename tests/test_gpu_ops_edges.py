@@ -137,3 +137,25 @@ def test_attention_scales_far_from_one(ops, dtype, d, scale):
     far_ds, far_dv = 2.0 ** -126 * 2800 * 2 * d * most * float(qkv[:, 2].abs().max()), 2.0 ** -126 * 50 * most
     hold([out, grads[1]], [want[0], (want[2][0], want[2][1] + far_ds)], f"{scale} {dtype}")
     hold([grads[0][:, 2]], [(want[1][0][:, 2], want[1][1][:, 2] + far_dv)], f"dv {scale} {dtype}")
+
+
+def test_lazily_negated_views(ops):
+    """x.conj().imag and torch._neg_view hold their values with the other sign in memory."""
+    g = torch.Generator().manual_seed(1)
+
+    def both(*shape):
+        z = torch.randn(*shape, dtype=torch.complex64, generator=g).cuda().conj().imag
+        n = torch._neg_view(torch.randn(*shape, generator=g).cuda())
+        assert z.is_neg() and n.is_neg()
+        return z, n
+    off, one = offsets_of([3, 4]), torch.ones(1, 1, device="cuda")
+    for x, w, b, r, q, t, do, dy, dm in zip(both(7, 1), both(1, 1), both(1), both(7, 1), both(7, 3, 1, 8), both(32, 1), both(7, 1, 8), both(7, 1), both(2, 1)):
+        plain = [v.clone().resolve_neg() for v in (x, w, b, r, q, t, do, dy, dm)]
+        outs = []
+        for x, w, b, r, q, t, do, dy, dm in ((x, w, b, r, q, t, do, dy, dm), plain):
+            leaf = [v.detach().clone().resolve_neg().requires_grad_() for v in (x, q)]
+            outs.append([ops.linear(x, w, b, "gelu", r), ops.bucketed_attention(q, t, off), ops.mean_pool(x, off, normalize=False),
+                         *torch.autograd.grad(ops.linear(leaf[0], one, None, "gelu"), [leaf[0]], dy),
+                         *torch.autograd.grad(ops.bucketed_attention(leaf[1], plain[5], off), [leaf[1]], do),
+                         *torch.autograd.grad(ops.mean_pool(leaf[0], off, normalize=False), [leaf[0]], dm)])
+        assert all(torch.equal(p, q) for p, q in zip(*outs))

@@ -93,6 +93,11 @@ def _first(t, name: str) -> int:
     return _DTYPES[t.dtype]
 
 
+def _whole(t: torch.Tensor) -> torch.Tensor:
+    """The tensor with its values in memory: a lazily negated view (x.conj().imag) holds them with the other sign."""
+    return t.resolve_neg() if t.is_neg() else t
+
+
 def _like(t, name: str, ref: torch.Tensor, shape) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor; got {type(t).__name__}")
@@ -112,6 +117,7 @@ def _check_offsets(offsets, ref: torch.Tensor) -> torch.Tensor:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """A matrix whose rows are dense and do not overlap: itself, or a copy."""
+    t = _whole(t)
     if t.is_contiguous():
         return t
     if t.stride(1) == 1 or t.shape[1] == 1:
@@ -203,7 +209,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     flat = x.dim() == 2
     x2 = _rows(x if flat else x.reshape(-1, k))
     w2 = _rows(weight)
-    b2 = None if bias is None else bias.contiguous()
+    b2 = None if bias is None else _whole(bias).contiguous()
     r2 = None if residual is None else _rows(residual if flat else residual.reshape(-1, n))
     act = ACTIVATIONS[activation]
     if _wants_grad(x, weight, bias, residual):
@@ -249,7 +255,7 @@ class _BucketedAttention(torch.autograd.Function):
         qkv, table, offsets, out, rest, lse = ctx.saved_tensors
         lib = _library()
         total, _, heads, d = qkv.shape
-        dout = dout.contiguous()
+        dout = _whole(dout).contiguous()
         dqkv = torch.empty((total, 3, heads, d), dtype=qkv.dtype, device=qkv.device)
         dtable = torch.empty_like(table) if ctx.needs_input_grad[1] else None
         size = lib.vdb_op_attention_backward_workspace_bytes(_DTYPES[qkv.dtype], offsets.shape[0] - 1, total, heads, d, table.shape[0])
@@ -281,7 +287,7 @@ def bucketed_attention(qkv: torch.Tensor, table: torch.Tensor, offsets: torch.Te
     scale = float(d) ** -0.5 if scale is None else float(scale)
     if qkv.stride(3) != 1 and d > 1 or min(qkv.stride()) < 0 or (heads > 1 and qkv.stride(2) < d):
         qkv = qkv.contiguous()
-    table = table.contiguous()
+    qkv, table = _whole(qkv), _whole(table).contiguous()
     if _wants_grad(qkv, table):
         return _BucketedAttention.apply(qkv, table, offsets, scale, int(max_distance))
     return _attention_forward(qkv, table, offsets, scale, int(max_distance), False)[0]
@@ -313,7 +319,7 @@ class _MeanPool(torch.autograd.Function):
     def backward(ctx, dy):
         y, inv, offsets = ctx.saved_tensors
         n, dim = y.shape
-        dy = dy.contiguous()
+        dy = _whole(dy).contiguous()
         dh = torch.empty((ctx.total, dim), dtype=ctx.dtype, device=y.device)
         _chk(_library().vdb_op_mean_pool_backward_dev(y.device.index, _DTYPES[ctx.dtype], dy.data_ptr(), y.data_ptr(), _ptr(inv), offsets.data_ptr(), n,
                                                       ctx.total, dim, int(ctx.normalize), dh.data_ptr(), _raw_stream(y.device.index)))
