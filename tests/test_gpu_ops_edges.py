@@ -159,3 +159,30 @@ def test_lazily_negated_views(ops):
                          *torch.autograd.grad(ops.bucketed_attention(leaf[1], plain[5], off), [leaf[1]], do),
                          *torch.autograd.grad(ops.mean_pool(leaf[0], off, normalize=False), [leaf[0]], dm)])
         assert all(torch.equal(p, q) for p, q in zip(*outs))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [24, 32, 64, 128])
+@pytest.mark.parametrize("value", [math.inf])
+def test_attention_infinity_in_the_table(ops, dtype, d, value):
+    """A bias of +inf makes every row NaN that meets its bucket (inf - inf), forward and back, and no other row or head."""
+    t = DT[dtype]
+    g = torch.Generator().manual_seed(d)
+    off = offsets_of([200, 1, 9])
+    qkv, table, dout = rnd(g, 210, 3, 2, d, dtype=t), rnd(g, 32, 2, dtype=t), rnd(g, 210, 2, d, dtype=t)
+
+    def both(tab):
+        leaf = qkv.cuda().requires_grad_()
+        out = ops.bucketed_attention(leaf, tab.cuda(), off)
+        dq, = torch.autograd.grad(out, [leaf], dout.cuda())
+        return out.detach().cpu(), dq[:, 0].cpu()
+    clean = both(table)
+    for bucket in (3, 15, 31):                       # at the diagonal, and both ends of the line
+        bad = table.clone()
+        bad[bucket, 1] = value
+        for got, want in zip(both(bad), clean):
+            assert torch.equal(got[:, 0], want[:, 0])
+            for lo, hi in ((0, 200), (200, 201), (201, 210)):
+                meets = (ref.buckets_of(hi - lo, 32, 128) == bucket).any(1)
+                assert torch.isnan(got[lo:hi][meets, 1]).all()
+                assert torch.equal(got[lo:hi][~meets], want[lo:hi][~meets])

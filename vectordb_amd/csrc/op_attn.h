@@ -480,6 +480,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams 
       const int e0 = j0 + u * 32 - i0;
       shift[u] = c * scores<T, D, KR, 1>(x[u], sk, u * 32, fq, e0, p, line, mid + e0);
       if (j0 + u * 32 + 32 > len) {
+        if (j0 + u * 32 >= len) shift[u] = 0.f;      // no key there meets a far bias, which may be NaN or infinite
 #pragma unroll
         for (int r = 0; r < 16; ++r) if (j0 + u * 32 + (r & 3) + 8 * (r >> 2) + 4 * half >= len) x[u][r] = -INFINITY;
       }
