@@ -163,9 +163,9 @@ def test_lazily_negated_views(ops):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("d", [24, 32, 64, 128])
-@pytest.mark.parametrize("value", [math.inf])
-def test_attention_infinity_in_the_table(ops, dtype, d, value):
-    """A bias of +inf makes every row NaN that meets its bucket (inf - inf), forward and back, and no other row or head."""
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_attention_nan_and_infinity_in_the_table(ops, dtype, d, value):
+    """A bias of NaN or +inf makes every row NaN that meets its bucket (inf - inf), forward and back, and no other row or head."""
     t = DT[dtype]
     g = torch.Generator().manual_seed(d)
     off = offsets_of([200, 1, 9])

@@ -341,7 +341,8 @@ __device__ __forceinline__ void make_start_line(float* line, const AttnParams& p
   const float most = 3e38f / fmaxf(c, 1.f);
   for (int t = threadIdx.x; t < p.n_buckets; t += blockDim.x) {
     const float b = (float)((const T*)p.table)[(long long)t * p.heads + head];
-    tab[t] = __builtin_isinf(b) ? b : fminf(fmaxf(b / p.scale, -most), most);
+    const float x = b / p.scale;
+    tab[t] = __builtin_isinf(b) ? b : x > most ? most : x < -most ? -most : x;       // NaN stays
   }
   __syncthreads();
   const int middle = start_zero(p.reach), w = around < middle ? around : middle;
