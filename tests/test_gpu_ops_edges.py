@@ -186,3 +186,63 @@ def test_attention_nan_and_infinity_in_the_table(ops, dtype, d, value):
                 meets = (ref.buckets_of(hi - lo, 32, 128) == bucket).any(1)
                 assert torch.isnan(got[lo:hi][meets, 1]).all()
                 assert torch.equal(got[lo:hi][~meets], want[lo:hi][~meets])
+
+
+@pytest.mark.parametrize("dtype,low", [("f32", torch.finfo(torch.float32).min), ("bf16", torch.finfo(torch.bfloat16).min), ("f32", -1e30), ("bf16", -1e11),
+                                       ("f32", 2e38), ("f16", -math.inf)])
+@pytest.mark.parametrize("d", [24, 32, 64, 128])
+@pytest.mark.parametrize("lengths", [[300, 1, 19, 70], [40] * 9], ids=["long", "short"])
+def test_attention_rows_of_one_great_bias(ops, dtype, low, d, lengths):
+    """Where every bias of a row is the same great number, the scores vanish beside it: p = 1 / length, forward and back.  (fp16's lowest value leaves
+    room for the scores in 32 bits; -inf leaves nothing of a row.)  The head beside it has ordinary biases."""
+    t, heads = DT[dtype], 2
+    g = torch.Generator().manual_seed(sum(lengths) + d)
+    total = sum(lengths)
+    qkv, table, dout = rnd(g, total, 3, heads, d, dtype=t), rnd(g, 32, heads, dtype=t), rnd(g, total, heads, d, dtype=t)
+    off = offsets_of(lengths)
+    great = table.clone()
+    great[:, 1] = low
+    lq, lt = qkv.cuda().requires_grad_(), great.cuda().requires_grad_()
+    out = ops.bucketed_attention(lq, lt, off)
+    dqkv, dtable = torch.autograd.grad(out, [lq, lt], dout.cuda())
+    # without q, or without k, the scores are 0 and so is what an even bias changes
+    flat = table.clone()
+    flat[:, 1] = 0
+    wants = []
+    for which in (0, 1):
+        x = qkv.clone()
+        x[:, which, 1] = 0
+        wants.append(ref.attention(x, flat, off.tolist(), d ** -0.5, 128, dout))
+    (o, g0, dt), g1 = wants[0], wants[1][1]
+    if low == -math.inf:
+        assert not out[:, 1].any() and not dqkv[:, :, 1].any() and not dtable[:, 1].any()
+        pick = slice(0, 1)
+    else:
+        pick = slice(0, 2)
+    hold([out[:, pick], dtable[:, pick]], [tuple(v[:, pick] for v in o), tuple(v[:, pick] for v in dt)], f"{dtype} {low}")
+    for i, w in ((0, g0), (1, g1), (2, g0)):         # dq holds k and no q, dk q and no k
+        for h in range(pick.stop):
+            if h == 0 or i != 1 or w is g1:
+                hold([dqkv[:, i, h]], [tuple(v[:, i, h] for v in w)], f"{dtype} {low} gradient {i} head {h}")
+
+
+@pytest.mark.parametrize("dtype,low", [("f32", torch.finfo(torch.float32).min), ("bf16", -1e9), ("bf16", torch.finfo(torch.bfloat16).min)])
+@pytest.mark.parametrize("d", [24, 32, 64, 128])
+def test_attention_one_row_left_to_great_biases(ops, dtype, low, d):
+    """Keys strictly before the query, by great negative biases: the first row of a text has none and takes all keys evenly, beside rows
+    that have some."""
+    t, n = DT[dtype], 150
+    g = torch.Generator().manual_seed(d)
+    qkv, table, dout = rnd(g, n, 3, 1, d, dtype=t), rnd(g, 32, 1, dtype=t), rnd(g, n, 1, d, dtype=t)
+    table[0], table[16:] = low, low
+    lq = qkv.cuda().requires_grad_()
+    out = ops.bucketed_attention(lq, table.cuda(), offsets_of([n]))
+    dqkv, = torch.autograd.grad(out, [lq], dout.cuda())
+    q, k, v = qkv[:, :, 0].double().unbind(1)
+    s = d ** -0.5 * (q @ k.t()) + table[:, 0].double()[ref.buckets_of(n, 32, 128)]
+    s[0] = 0
+    p, go = torch.softmax(s, 1), dout[:, 0].double()
+    # scores of size 5 are off by (d + 20) E 5 in the exponent; p, rounded to 16 bits, by u; the sums by (n + d) E; the result by u
+    u = ref.half_step(t)
+    rel = (2 * u if dtype != "f32" else u) + (n + 12 * (d + 20)) * ref.E
+    hold([out[:, 0], dqkv[:, 2, 0]], [(p @ v, rel * (p @ v.abs()) + 2.0 ** -126), (p.t() @ go, rel * (p.t() @ go.abs()) + 2.0 ** -120)], f"{dtype} {low}")

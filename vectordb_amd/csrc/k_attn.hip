@@ -37,10 +37,6 @@ unsigned hop_of(unsigned n) {
   return 1;
 }
 
-// The tiled kernels let the bias enter a product that is scaled afterwards, as bias / scale: with a scale far from 1 that quotient leaves
-// the 32-bit range (100 / 1e-37) or its normal part, and the bias would be lost.  The general kernels add it behind the scaling.
-bool even_scale(float s) { return s >= 1e-18f && s <= 1e18f; }
-
 template <typename T, int DP, int NW>
 hipError_t forward(const AttnParams& p, hipStream_t st) {
   const unsigned slots = (unsigned)n_slots(p.total, p.n_seqs, NW * 32), grid = slots * p.heads;
@@ -107,7 +103,7 @@ hipError_t run_dp(const AttnParams& p, const AttnArgs& a, bool back) {
 template <typename T>
 hipError_t run_t(const AttnArgs& a, bool back) {
   AttnParams p = params(a, sizeof(T));
-  p.delta = a.delta; p.part = a.part; p.peak = (const unsigned*)a.gscale; p.order = (const i32x4*)a.order;
+  p.delta = a.delta; p.fix = a.fix; p.part = a.part; p.peak = (const unsigned*)a.gscale; p.order = (const i32x4*)a.order;
   if (back) {
     const unsigned grid = (unsigned)(n_slots(p.total, p.n_seqs, 32) * p.heads);
     if (a.gscale) {
@@ -132,12 +128,14 @@ hipError_t launch_attention(int dtype, const AttnArgs& a) {
 
 int64_t attention_backward_workspace(int dtype, int64_t n_seqs, int64_t total, int heads, int d, int n_buckets) {
   const int64_t slots = n_slots(total, n_seqs, 32 * tile_waves(dtype, d, true, n_seqs, total));
-  return pad256(total * heads * 4) + (dtype == 2 ? pad256(2 * n_seqs * heads * 4) : 0) + pad256(slots * heads * n_buckets * 4) +
+  return 2 * pad256(total * heads * 4) + (dtype == 2 ? pad256(2 * n_seqs * heads * 4) : 0) + pad256(slots * heads * n_buckets * 4) +
          (by_length(n_seqs, total, slots, heads) ? pad256(slots * 16) : 0);
 }
 
 hipError_t launch_attention_backward(int dtype, AttnArgs a, char* ws) {
   a.delta = (float*)ws;
+  ws += pad256(a.total * a.heads * 4);
+  a.fix = (float*)ws;
   ws += pad256(a.total * a.heads * 4);
   a.gscale = nullptr;
   if (dtype == 2) { a.gscale = (float*)ws; ws += pad256(2 * a.n_seqs * a.heads * 4); }

@@ -23,7 +23,7 @@ struct AttnParams {
   int heads, d; float scale;
   void* out; void* rest; float* lse;
   const void* dout; void *dq, *dk, *dv; long long gld_t, gld_h;
-  float* delta; const unsigned* peak; float* part;   // peak: [2][heads][n_seqs] largest |dout| and |v| (fp16 only)
+  float* delta; float* fix; const unsigned* peak; float* part;   // peak: [2][heads][n_seqs] largest |dout| and |v| (fp16 only)
   const i32x4* order;   // the tiled backward kernels' places, longest sequences first, or nullptr
   int vec;        // q, k, v, out, dout, gradients: 16-byte rows
   int reach;      // R
@@ -43,17 +43,38 @@ __device__ __forceinline__ int bucket_of(const Buckets& bk, int e) {
   return b + (e > 0 ? bk.half : 0);
 }
 
-// line[R + e] = bias(e) * log2(e) for |e| <= R.  A finite bias stays finite: the product of the type's lowest value with
-// log2(e) would be -inf and a row of such values would lose its softmax.
+// The tiled kernels let the bias enter a product that is scaled afterwards, as bias / scale: with a scale far from 1 that quotient leaves
+// the 32-bit range (100 / 1e-37) or its normal part, and the bias would be lost.  Then the general kernels serve, which add it behind the
+// scaling.
+__host__ __device__ __forceinline__ bool even_scale(float s) { return s >= 1e-18f && s <= 1e18f; }
+// What the bias b is in such a product, c = scale log2(e).  Finite values stay within what the product with c can hold: a row of the
+// type's lowest value has a softmax.  NaN stays.
+__device__ __forceinline__ float start_value(float b, float scale, float c) {
+  const float most = 3e38f / fmaxf(c, 1.f), x = b / scale;
+  return __builtin_isinf(b) ? b : x > most ? most : x < -most ? -most : x;
+}
+
+// line[R + e] = bias(e) * log2(e) for |e| <= R: by the same steps as in the tiled kernels where they may have made the other pass (fp32
+// heads of 128), so that great biases come out as the same numbers in both.
 template <typename T>
 __device__ __forceinline__ void make_line(float* line, const AttnParams& p, int head) {
+  const float c = p.scale * kLog2e;
   for (int t = threadIdx.x; t <= 2 * p.reach; t += blockDim.x) {
     const float b = (float)((const T*)p.table)[(long long)bucket_of(p.bk, t - p.reach) * p.heads + head];
     float x = b * kLog2e;
     if (__builtin_isinf(x) && !__builtin_isinf(b)) x = b < 0.f ? -3.4028234e38f : 3.4028234e38f;
-    line[t] = x;
+    line[t] = even_scale(p.scale) ? start_value(b, p.scale, c) * c : x;
   }
 }
+
+// Rows whose scores lie beyond 2^10 (all of a row's biases are some mask's great number) take a slower, exact way through exp2(s - m):
+// - s is rounded before m is taken away.  Fused, scale x - m keeps the product's exact tail, and half a step of a number like 1e38 is far
+//   beyond any exponent.
+// - The kept lse = m + log2(sum) has no room for log2(sum) there (at the type's lowest value p would be 1 instead of 1 / len): the backward
+//   pass sums the row's exp2(s - lse) once more and takes log2 of that away too (`fix`, 0 for other rows).
+// The tiled kernels do so in a branch ahead of the exponentials that turns a tile's x into (s - m) / c, so that what every tile runs
+// through stays as it is: with a second form of the exponentials in the loop, 16 x 384 tokens in fp32 took 107 us instead of 85.
+__device__ __forceinline__ bool is_great(float x) { return fabsf(x) > 1024.f && fabsf(x) < INFINITY; }
 
 // ROWS rows of one head into LDS: [ROWS][DP + V], or transposed [DP][ROWS + V]; zeros beyond `valid` rows and d columns.
 template <typename T, int DP, int ROWS, bool PLAIN, bool TRANS>
@@ -332,18 +353,12 @@ __device__ __forceinline__ void add_across(f32x16 (&acc)[D / 32], const T* s, in
 }
 
 // line[start_at(R, e)] = bias(e) / scale, |e| <= R + kMargin: the start value of a tile's sums, so that a tile near the diagonal costs a
-// look-up a score and no arithmetic.  Finite values stay within what the later product with scale log2(e) can hold: a row
-// of the type's lowest value has a softmax.  Only the distances that a text of this length meets are filled in (around: its length and
+// look-up a score and no arithmetic.  Only the distances that a text of this length meets are filled in (around: its length and
 // a tile; a far tile, which takes its bias from an end of the line, is met only where all of it is).
 template <typename T>
 __device__ __forceinline__ void make_start_line(float* line, const AttnParams& p, int head, float c, int around) {
   __shared__ float tab[128];
-  const float most = 3e38f / fmaxf(c, 1.f);
-  for (int t = threadIdx.x; t < p.n_buckets; t += blockDim.x) {
-    const float b = (float)((const T*)p.table)[(long long)t * p.heads + head];
-    const float x = b / p.scale;
-    tab[t] = __builtin_isinf(b) ? b : x > most ? most : x < -most ? -most : x;       // NaN stays
-  }
+  for (int t = threadIdx.x; t < p.n_buckets; t += blockDim.x) tab[t] = start_value((float)((const T*)p.table)[(long long)t * p.heads + head], p.scale, c);
   __syncthreads();
   const int middle = start_zero(p.reach), w = around < middle ? around : middle;
   for (int t = middle - w + threadIdx.x; t <= middle + w; t += blockDim.x) line[t] = tab[bucket_of(p.bk, t - middle)];
@@ -463,7 +478,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams 
   const float* mid = line + start_at(p.reach, 4 * half - l);      // mid[e0 + row] = start value of row (+ 4 half), column l
 #pragma unroll
   for (int x = 0; x < D / (2 * V); ++x) settle(fq[x]);
-  float m = -INFINITY, sum = 0.f;
+  float m = -INFINITY, base = 0.f, sum = 0.f;
+  bool great = false;                  // some row of the wave has a great maximum
   f32x16 acc[D / 32] = {};
   for (int t = 0; t < tiles; ++t) {
     wait_loads<0>();
@@ -488,17 +504,27 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams 
       float high = x[u][0];
 #pragma unroll
       for (int r = 1; r < 16; ++r) high = fmaxf(high, x[u][r]);
-      top = fmaxf(top, high * c + shift[u]);
+      top = fmaxf(top, __builtin_fmaf(high, c, shift[u]));
     }
     top = fmaxf(top, __shfl_xor(top, 32, 64));
-    if (__any(top > m)) {
+    if (__any(top > m) || great) {
       const float m1 = fmaxf(m, top), fade = __builtin_amdgcn_exp2f(m - (m1 == -INFINITY ? 0.f : m1));
       m = m1;
+      base = m == -INFINITY ? 0.f : m;       // a row of -inf alone: p = 0, not NaN
       sum *= fade;
 #pragma unroll
       for (int db = 0; db < D / 32; ++db) acc[db] *= fade;
+      great = __any(is_great(m));
+      if (great) {
+#pragma unroll
+        for (int u = 0; u < KT / 32; ++u) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) x[u][r] = (__builtin_fmaf(x[u][r], c, shift[u]) - base) / c;
+          shift[u] = 0.f;
+        }
+        base = 0.f;
+      }
     }
-    const float base = m == -INFINITY ? 0.f : m;       // a row of -inf alone: p = 0, not NaN
 #pragma unroll
     for (int u = 0; u < KT / 32; ++u) {
       const float off = shift[u] - base;
@@ -670,6 +696,22 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_any_kernel(const AttnPar
   const float delta = i < len ? p.delta[(long long)head * p.total + s.begin + i] : 0.f;
   const float lift = ds_lift<T>(p, head, s.b);
   const float c = p.scale * kLog2e;
+  float fix = 0.f;
+  if (__builtin_amdgcn_readfirstlane(__syncthreads_or(is_great(lse)))) {
+    float sum = 0.f;
+    for (int j0 = 0; j0 < len; j0 += 32) {
+      __syncthreads();
+      stage_rows<T, DP, 32, true, false>(sk, nullptr, kb + j0 * p.ld_t, p.ld_t, len - j0, p.d, p.vec, NW * 64);
+      __syncthreads();
+      f32x16 t = rows_times<T, DP>(sk, fq);
+      add_bias<true>(t, c, line, reach, j0 - i0);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) if (j0 + (r & 3) + 8 * (r >> 2) + 4 * half < len) sum += __builtin_amdgcn_exp2f(t[r] - lse);
+    }
+    sum += __shfl_xor(sum, 32, 64);
+    if (is_great(lse)) fix = log2f(sum);
+  }
+  if (lane < 32 && i < len) p.fix[(long long)head * p.total + s.begin + i] = fix;
   float below = 0.f, above = 0.f;
   f32x16 acc[DP / 32] = {};
   for (int j0 = 0; j0 < len; j0 += 32) {
@@ -685,7 +727,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_any_kernel(const AttnPar
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int j = j0 + (r & 3) + 8 * (r >> 2) + 4 * half;
-      const float w = j < len ? __builtin_amdgcn_exp2f(t[r] - lse) : 0.f;
+      const float w = j < len ? __builtin_amdgcn_exp2f(t[r] - lse - fix) : 0.f;
       t[r] = w == 0.f ? 0.f : w * (dp[r] - delta);
     }
     if constexpr (DTABLE) {
@@ -717,7 +759,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_any_kernel(const AttnPa
   __shared__ __align__(16) T sqt[DP * (32 + V)];
   __shared__ __align__(16) T sg[32 * (DP + V)];
   __shared__ __align__(16) T sgt[DP * (32 + V)];
-  __shared__ __align__(16) float sl[32], sd[32];
+  __shared__ __align__(16) float sl[32], sd[32], sf[32];
   extern __shared__ float line[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
   const int head = blockIdx.x % p.heads;
@@ -740,6 +782,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_any_kernel(const AttnPa
   const T* gb = (const T*)p.dout + s.begin * hd + (long long)head * p.d;
   const float* lse = p.lse + (long long)head * p.total + s.begin;
   const float* delta = p.delta + (long long)head * p.total + s.begin;
+  const float* fix = p.fix + (long long)head * p.total + s.begin;
   const float lift = ds_lift<T>(p, head, s.b);
   const float c = p.scale * kLog2e;
   f32x16 ak[DP / 32] = {}, av[DP / 32] = {};
@@ -750,6 +793,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_any_kernel(const AttnPa
     if (threadIdx.x < 32) {
       sl[threadIdx.x] = i0 + (int)threadIdx.x < len ? lse[i0 + threadIdx.x] : INFINITY;
       sd[threadIdx.x] = i0 + (int)threadIdx.x < len ? delta[i0 + threadIdx.x] : 0.f;
+      sf[threadIdx.x] = i0 + (int)threadIdx.x < len ? fix[i0 + threadIdx.x] : 0.f;
     }
     __syncthreads();
     if (j0 >= len) continue;
@@ -760,7 +804,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_any_kernel(const AttnPa
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int row = (r & 3) + 8 * (r >> 2) + 4 * half;
-      t[r] = __builtin_amdgcn_exp2f(t[r] - sl[row]);
+      t[r] = __builtin_amdgcn_exp2f(t[r] - sl[row] - sf[row]);
       ds[r] = t[r] == 0.f ? 0.f : t[r] * (dp[r] - sd[row]);
     }
     trans_times<T, DP>(av, sgt, t);
@@ -905,6 +949,32 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
   float from = -lse, less = delta;
   settle(from);
   settle(less);
+  float fix = 0.f;
+  const bool great = __builtin_amdgcn_readfirstlane(__syncthreads_or(is_great(lse)));
+  if (great) {
+    float sum = 0.f;
+    for (int t = 0; t < tiles; ++t) {
+      wait_loads<0>();
+      __syncthreads();
+      if (t + 1 < tiles) issue(t + 1);
+      if (i0 >= len) continue;
+#pragma unroll 1
+      for (int u = 0; u < KT / 32; ++u) {
+        const int j0 = t * KT + u * 32, e0 = j0 - i0;
+        if (j0 >= len) break;
+        f32x16 x;
+        const float bias = c * scores<T, D, R, 1>(x, buf[t & 1][0], u * 32, fq, e0, p, line, mid + e0);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (j0 + (r & 3) + 8 * (r >> 2) + 4 * half < len) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], c, bias) + from);
+      }
+    }
+    sum += __shfl_xor(sum, 32, 64);
+    if (is_great(lse)) fix = log2f(sum);
+    __syncthreads();                 // the last tile is read: its place may be loaded again
+    issue(0);
+  }
+  if (lane < 32 && i0 + l < len) p.fix[row] = fix;
   float below = 0.f, above = 0.f;
   f32x16 acc[D / 32] = {};
   for (int t = 0; t < tiles; ++t) {
@@ -920,7 +990,14 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
       if (j0 >= len) break;
       const bool is_far = tile_is_far(e0, reach);
       f32x16 x, dp = {};
-      const float shift = from + c * scores<T, D, R, 1>(x, sk, u * 32, fq, e0, p, line, mid + e0);
+      float shift = c * scores<T, D, R, 1>(x, sk, u * 32, fq, e0, p, line, mid + e0);
+      if (great) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = (__builtin_fmaf(x[r], c, shift) + from - fix) / c;
+        shift = 0.f;
+      } else {
+        shift += from;
+      }
 #pragma unroll
       for (int y = 0; y < D / (2 * V); ++y) Elem<T>::mma(RV::along(sv, u * 32, y), fg[y], dp);
 #pragma unroll
@@ -964,7 +1041,8 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
   using R = Rows<T, D, kCol>;
   using vec = typename Elem<T>::vec;
   __shared__ __align__(1024) T buf[2][2][QT * D];       // [turn][q, dout]
-  __shared__ __align__(16) float stat[2][2][QT];             // [turn][lse, delta]
+  __shared__ __align__(16) float stat[2][4][QT];             // [turn][lse (a great tile: 0), delta, a great tile: lse, fix]
+  __shared__ int some_great[2];                              // [turn]: whether any of the tile's queries is
   extern __shared__ float line[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l = lane & 31;
   int head;
@@ -984,7 +1062,8 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
   const T* gb = (const T*)p.dout + s.begin * hd + (long long)head * D;
   const float* lse = p.lse + (long long)head * p.total + s.begin;
   const float* delta = p.delta + (long long)head * p.total + s.begin;
-  float next_lse = 0.f, next_delta = 0.f;    // thread x < QT: of query x of the tile under way
+  const float* fix = p.fix + (long long)head * p.total + s.begin;
+  float next_lse = 0.f, next_delta = 0.f, next_fix = 0.f;    // thread x < QT, the first wave: of query x of the tile under way
   auto issue = [&](int t) {
     const int left = len - t * QT;
     R::template load<QT, NW * 64>(buf[t & 1][0], qb + (long long)t * QT * p.ld_t, p.ld_t, left);
@@ -993,6 +1072,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
       const bool there = (int)threadIdx.x < left;
       next_lse = there ? lse[t * QT + threadIdx.x] : INFINITY;
       next_delta = there ? delta[t * QT + threadIdx.x] : 0.f;
+      next_fix = there ? fix[t * QT + threadIdx.x] : 0.f;
     }
   };
   issue(0);
@@ -1012,19 +1092,35 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
   for (int x = 0; x < D / (2 * V); ++x) { settle(fk[x]); settle(fv[x]); }
   f32x16 ak[D / 32] = {}, av[D / 32] = {};
   for (int t = 0; t < tiles; ++t) {
-    if (threadIdx.x < QT) { stat[t & 1][0][threadIdx.x] = next_lse; stat[t & 1][1][threadIdx.x] = next_delta; }
+    if (threadIdx.x < QT) {
+      const bool any = __any(is_great(next_lse));
+      stat[t & 1][0][threadIdx.x] = any ? 0.f : next_lse;
+      stat[t & 1][1][threadIdx.x] = next_delta;
+      stat[t & 1][2][threadIdx.x] = next_lse;
+      stat[t & 1][3][threadIdx.x] = next_fix;
+      if (threadIdx.x == 0) some_great[t & 1] = any;
+    }
     wait_loads<0>();
     __syncthreads();
     if (t + 1 < tiles) issue(t + 1);
     if (j0 >= len) continue;
     const T* sq = buf[t & 1][0];
     const T* sg = buf[t & 1][1];
+    const bool great = __builtin_amdgcn_readfirstlane(some_great[t & 1]);
 #pragma unroll 1
     for (int u = 0; u < QT / 32; ++u) {
       if (t * QT + u * 32 >= len) break;
       const int e0 = j0 - t * QT - u * 32;
       f32x16 x, dp = {};
-      const float shift = c * scores<T, D, R, -1>(x, sq, u * 32, fk, e0, p, line, mid + e0);
+      float shift = c * scores<T, D, R, -1>(x, sq, u * 32, fk, e0, p, line, mid + e0);
+      if (great) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int row = u * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
+          x[r] = (__builtin_fmaf(x[r], c, shift) - stat[t & 1][2][row] - stat[t & 1][3][row]) / c;
+        }
+        shift = 0.f;
+      }
 #pragma unroll
       for (int y = 0; y < D / (2 * V); ++y) Elem<T>::mma(R::along(sg, u * 32, y), fv[y], dp);
 #pragma unroll
