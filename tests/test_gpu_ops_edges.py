@@ -246,3 +246,24 @@ def test_attention_one_row_left_to_great_biases(ops, dtype, low, d):
     u = ref.half_step(t)
     rel = (2 * u if dtype != "f32" else u) + (n + 12 * (d + 20)) * ref.E
     hold([out[:, 0], dqkv[:, 2, 0]], [(p @ v, rel * (p @ v.abs()) + 2.0 ** -126), (p.t() @ go, rel * (p.t() @ go.abs()) + 2.0 ** -120)], f"{dtype} {low}")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [24, 32, 64, 128])
+@pytest.mark.parametrize("size", [1e4, 1e9, 1e15])
+def test_attention_great_scores(ops, dtype, d, size):
+    """Scores of 1e8 to 1e31: each row is the value of its greatest score, to the bit (where no other comes within the sums' rounding)."""
+    t, n = DT[dtype], 150
+    g = torch.Generator().manual_seed(d)
+    qkv, table, dout = rnd(g, n, 3, 1, d, dtype=t), rnd(g, 32, 1, dtype=t), rnd(g, n, 1, d, dtype=t)
+    qkv[:, :2] *= size
+    q, k, v = qkv[:, :, 0].double().unbind(1)
+    s = q @ k.t()
+    top = s.topk(2, 1)
+    clear = top.values[:, 0] - top.values[:, 1] > 2 * (d + 6) * ref.E * (q.abs() @ k.abs().t()).max(1).values + 1e3
+    assert clear.sum() > n * 3 // 4
+    lq = qkv.cuda().requires_grad_()
+    out = ops.bucketed_attention(lq, table.cuda(), offsets_of([n]))
+    assert torch.isfinite(out).all() and torch.equal(out.detach().cpu()[clear, 0], qkv[top.indices[clear, 0], 2, 0])
+    dqkv, = torch.autograd.grad(out, [lq], dout.cuda())
+    assert torch.isfinite(dqkv).all()
