@@ -127,6 +127,31 @@ def test_buckets_are_the_models_whatever_its_table():
         encoder_of(model_of(relative_attention_num_buckets=16))
 
 
+def test_layers_that_are_no_plain_products_are_refused():
+    """An adapter around a layer computes more than its weight says; a parametrised layer's weight is what it computes."""
+    class Adapted(torch.nn.Linear):
+        def forward(self, x):
+            return super().forward(x) + 1.0
+
+    class Doubled(torch.nn.Module):
+        def forward(self, w):
+            return 2 * w
+    model = model_of()
+    enc = encoder_of(model)
+    q = model.encoder.layer[1].attention.attn.q
+    model.encoder.layer[1].attention.attn.q = Adapted(q.in_features, q.out_features)
+    for grad in (False, True):
+        with pytest.raises(ValueError, match="Adapted"):
+            vectors(enc, grad)
+    model.encoder.layer[1].attention.attn.q = q
+    before = vectors(enc)
+    torch.nn.utils.parametrize.register_parametrization(model.encoder.layer[0].output.dense, "weight", Doubled())
+    assert not torch.equal(vectors(enc), before) and float((vectors(enc) - models_own(model)).abs().max()) < 2e-6
+    from transformers import BertConfig, BertModel
+    with pytest.raises(ValueError, match="BertModel"):
+        encoder_of(BertModel(BertConfig(vocab_size=20, hidden_size=16, num_hidden_layers=1, num_attention_heads=2, intermediate_size=16)))
+
+
 def test_nothing_is_kept_between_calls():
     """No tensor outlives a call, so no later call on another stream, and no captured graph, can meet one that is unwritten or freed."""
     enc = encoder_of(model_of(), torch.bfloat16)

@@ -27,6 +27,8 @@ class MPNetEncoder:
 
     def __init__(self, model: torch.nn.Module, dtype: torch.dtype = torch.float32):
         cfg = model.config
+        if getattr(cfg, "model_type", None) != "mpnet":
+            raise ValueError(f"only MPNet models are supported; got {type(model).__name__}")
         if cfg.hidden_act not in _ACTIVATIONS:
             raise ValueError(f"hidden_act {cfg.hidden_act!r} is not one of {sorted(_ACTIVATIONS)}")
         if cfg.hidden_size % cfg.num_attention_heads or cfg.hidden_size // cfg.num_attention_heads > 128:
@@ -45,7 +47,11 @@ class MPNetEncoder:
     def _modules(self):
         for layer in self.model.encoder.layer:
             a = layer.attention.attn
-            yield a, layer.attention.LayerNorm, layer.intermediate.dense, layer.output.dense, layer.output.LayerNorm
+            up, down = layer.intermediate.dense, layer.output.dense
+            for m in (a.q, a.k, a.v, a.o, up, down):
+                if type(m).forward is not torch.nn.Linear.forward:     # an adapter or a quantised layer: its weight alone is not what it computes
+                    raise ValueError(f"layers must be torch.nn.Linear; got {type(m).__name__}")
+            yield a, layer.attention.LayerNorm, up, down, layer.output.LayerNorm
 
     def _table(self):
         return self.model.encoder.relative_attention_bias.weight[:BUCKETS]
