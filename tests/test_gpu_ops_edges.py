@@ -267,3 +267,22 @@ def test_attention_great_scores(ops, dtype, d, size):
     assert torch.isfinite(out).all() and torch.equal(out.detach().cpu()[clear, 0], qkv[top.indices[clear, 0], 2, 0])
     dqkv, = torch.autograd.grad(out, [lq], dout.cuda())
     assert torch.isfinite(dqkv).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_relu_lets_no_infinity_back(ops, dtype):
+    """Where relu's sum is not positive its gradient is 0, whatever arrives there."""
+    t = DT[dtype]
+    for m, n, k in ((5, 3, 4), (300, 136, 40)):
+        g = torch.Generator().manual_seed(m)
+        x, w = rnd(g, m, k, dtype=t), rnd(g, n, k, dtype=t)
+        z = x.double() @ w.double().t()
+        dy = rnd(g, m, n, dtype=t)
+        clean, dirty = dy.masked_fill(z < -0.1, 0.0), dy.masked_fill(z < -0.1, math.inf)
+        dirty[z < -1] = math.nan
+        b = torch.zeros(n, dtype=t)
+        grads = []
+        for d in (clean, dirty):
+            leaves = [v.cuda().requires_grad_() for v in (x, w, b)]
+            grads.append(torch.autograd.grad(ops.linear(leaves[0], leaves[1], leaves[2], "relu"), leaves, d.cuda()))
+        assert all(torch.equal(p, q) for p, q in zip(*grads))

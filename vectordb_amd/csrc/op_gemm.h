@@ -523,7 +523,8 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ dy,
     for (long long i = r0 + wave; i < r1; i += 4) {
       float g = (float)dy[i * lddy + j];
       if constexpr (ACT != 0) {
-        g *= act_slope<T, ACT>((float)z[i * n + j]);
+        const float slope = act_slope<T, ACT>((float)z[i * n + j]);
+        g = ACT == 3 && slope == 0.f ? 0.f : g * slope;      // relu lets nothing through, an infinity or NaN neither
         if (dz) dz[i * n + j] = (T)g;
       }
       s += g;
