@@ -51,6 +51,20 @@ def test_gives_the_models_vectors():
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("own", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("layers", [1, 3])
+def test_numbers_of_layers_and_types_of_models(dtype, own, layers):
+    """With and without gradients the same, whatever type the model's parameters have."""
+    model = model_of(num_hidden_layers=layers).to(own)
+    enc = encoder_of(model, dtype)
+    got = vectors(enc)
+    assert got.dtype == torch.float32 and torch.equal(got, vectors(enc, grad=True).detach())
+    # 16-bit layers: three roundings of half a step a product, unit vectors of 32 values after at most three layers
+    wide = vectors(encoder_of(model.float()))
+    assert float((got - wide).abs().max()) < (2e-6 if dtype == torch.float32 else 0.05)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("how", ["sgd", "fused adamw", "replaced parameters", "data", "inference tensors", "another model's weights"])
 def test_every_change_of_the_weights_shows(dtype, how):
     """Whatever changes the parameters, the next call without gradients computes with what they hold then: fused optimisers and writes

@@ -132,7 +132,7 @@ class MPNetEncoder:
         parameters (unless weights, of lay_out(), are given)."""
         emb = self.model.embeddings
         table, layers = weights or (self._layers() if torch.is_grad_enabled() else self.lay_out())
-        x = (emb.word_embeddings(ids) + emb.position_embeddings(places)).float()
+        x = emb.word_embeddings(ids).float() + emb.position_embeddings(places).float()
         hidden = x.shape[1]
         x = F.layer_norm(x, (hidden,), emb.LayerNorm.weight.float(), emb.LayerNorm.bias.float(), self.eps)
         for wqkv, bqkv, wo, bo, g1, c1, w1, b1, w2, b2, g2, c2 in layers:
