@@ -52,9 +52,9 @@ def test_gives_the_models_vectors():
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("own", [torch.float32, torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("layers", [1, 3])
+@pytest.mark.parametrize("layers", [0, 1, 3])
 def test_numbers_of_layers_and_types_of_models(dtype, own, layers):
-    """With and without gradients the same, whatever type the model's parameters have."""
+    """With and without gradients the same, whatever type the model's parameters have; no layers at all, too."""
     model = model_of(num_hidden_layers=layers).to(own)
     enc = encoder_of(model, dtype)
     got = vectors(enc)

@@ -98,11 +98,12 @@ class MPNetEncoder:
                 layers.append((copied(a.q.weight, a.k.weight, a.v.weight), copied(a.q.bias, a.k.bias, a.v.bias),
                                taken(a.o.weight), taken(a.o.bias), norm.weight.float(), norm.bias.float(), taken(up.weight), taken(up.bias),
                                taken(down.weight), taken(down.bias), norm2.weight.float(), norm2.bias.float()))
-            flat = torch.empty(at, dtype=dt, device=sources[0].device)
+            flat = torch.empty(at, dtype=dt, device=self._table().device)
 
             def view(begin, shape):
                 return flat.as_strided(shape, (shape[1], 1) if len(shape) == 2 else (1,), begin)
-            torch._foreach_copy_([view(b, p.shape) for b, p in zip(places, sources)], sources)
+            if sources:
+                torch._foreach_copy_([view(b, p.shape) for b, p in zip(places, sources)], sources)
             return (table if isinstance(table, torch.Tensor) else view(*table),
                     [tuple(w if isinstance(w, torch.Tensor) else view(*w) for w in layer) for layer in layers])
 
