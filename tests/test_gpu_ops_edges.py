@@ -286,3 +286,29 @@ def test_relu_lets_no_infinity_back(ops, dtype):
             leaves = [v.cuda().requires_grad_() for v in (x, w, b)]
             grads.append(torch.autograd.grad(ops.linear(leaves[0], leaves[1], leaves[2], "relu"), leaves, d.cuda()))
         assert all(torch.equal(p, q) for p, q in zip(*grads))
+
+
+@pytest.mark.parametrize("d", [24, 32, 64, 128])
+@pytest.mark.parametrize("small", [1.37 * 2.0 ** -18, 1.37 * 2.0 ** -23, 1.37 * 2.0 ** -26])
+def test_attention_small_probabilities_keep_their_bits_in_fp16(ops, d, small):
+    """Beside a key that holds nearly all of a row's weight, probabilities of 2^-18 to 2^-26: forward and in v's gradient as close as an fp16
+    rounding of a normal number."""
+    n, u = 500, ref.half_step(torch.float16)
+    qkv = torch.zeros(n, 3, 1, d, dtype=torch.float16)
+    qkv[:, 0, 0, 0] = 8
+    qkv[7, 1, 0, 0] = -math.log(small) / 8 * math.sqrt(d)
+    qkv[:, 2] = 2.0 ** 14
+    qkv[7, 2] = 0
+    dout = torch.zeros(n, 1, d, dtype=torch.float16)
+    dout[0] = 2.0 ** 14
+    small = math.exp(-8 * float(qkv[7, 1, 0, 0]) / math.sqrt(d))        # of the key as it is rounded
+    p = small / (1 + (n - 1) * small)
+    leaf = qkv.cuda().requires_grad_()
+    out = ops.bucketed_attention(leaf, torch.zeros(32, 1, dtype=torch.float16, device="cuda"), offsets_of([n]))
+    dv = torch.autograd.grad(out, [leaf], dout.cuda())[0][:, 2].cpu().double()
+    keep = [i for i in range(n) if i != 7]
+    # scores of size s are off by (d + 20) E s in the exponent; p by u (2^-29 of the greatest is the last normal one), the results by u or, as subnormals, 2^-25
+    rel = 2 * u + 20 * (d + 20) * ref.E + n * ref.E
+    part = (n - 1) * p * 2.0 ** 14
+    assert ((out.detach().cpu().double() - part).abs() <= rel * part + 2.0 ** -25).all()
+    assert ((dv[keep] - p * 2.0 ** 14).abs() <= rel * p * 2.0 ** 14 + 2.0 ** -25).all()

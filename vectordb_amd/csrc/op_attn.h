@@ -76,6 +76,12 @@ __device__ __forceinline__ void make_line(float* line, const AttnParams& p, int 
 // through stays as it is: with a second form of the exponentials in the loop, 16 x 384 tokens in fp32 took 107 us instead of 85.
 __device__ __forceinline__ bool is_great(float x) { return fabsf(x) > 1024.f && fabsf(x) < INFINITY; }
 
+// fp16 operands: p <= 1 would lose bits below 2^-14 and vanish below 2^-25 (beside a key of nearly all the weight, or 1 / len of a text of
+// 20 thousand tokens); as 2^15 p it keeps them down to 2^-29.  The sums carry the factor too, dv and ds are freed of it.
+template <typename T> constexpr bool kLifted = sizeof(T) == 2 && !__is_same(T, __bf16);
+template <typename T> constexpr float kLift = kLifted<T> ? 15.f : 0.f;      // log2
+template <typename T> constexpr float kUnlift = kLifted<T> ? 1.f / 32768.f : 1.f;
+
 // ROWS rows of one head into LDS: [ROWS][DP + V], or transposed [DP][ROWS + V]; zeros beyond `valid` rows and d columns.
 template <typename T, int DP, int ROWS, bool PLAIN, bool TRANS>
 __device__ __forceinline__ void stage_rows(T* s, T* st, const T* g, long long ld, int valid, int d, int vec_ok, int threads) {
@@ -262,7 +268,7 @@ __global__ __launch_bounds__(NW * 64) void attention_any_kernel(const AttnParams
     const float fade = __builtin_amdgcn_exp2f(m - ms);
     l *= fade;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) { t[r] = __builtin_amdgcn_exp2f(t[r] - ms); l += t[r]; }
+    for (int r = 0; r < 16; ++r) { t[r] = __builtin_amdgcn_exp2f(t[r] - ms + kLift<T>); l += t[r]; }
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) acc[db] *= fade;
     trans_times<T, DP>(acc, sv, t);
@@ -274,7 +280,7 @@ __global__ __launch_bounds__(NW * 64) void attention_any_kernel(const AttnParams
   store_cols<T, DP>((T*)p.out + (s.begin + i) * hd + (long long)head * p.d, acc, f, p.d, p.vec);
   if (p.rest) store_cols<T, DP, true>((T*)p.rest + (s.begin + i) * hd + (long long)head * p.d, acc, f, p.d, p.vec);
   // +inf where nothing was left of the row: the backward pass' exp2(s - lse) is 0 there
-  if (p.lse && lane < 32) p.lse[(long long)head * p.total + s.begin + i] = l > 0.f || l != l ? m + log2f(l) : INFINITY;
+  if (p.lse && lane < 32) p.lse[(long long)head * p.total + s.begin + i] = l > 0.f || l != l ? m + (log2f(l) - kLift<T>) : INFINITY;
 }
 
 // ---- whole 16-byte pieces and head widths of 32, 64 and 128 ----------------------------------------------------------------
@@ -519,15 +525,15 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams 
 #pragma unroll
         for (int u = 0; u < KT / 32; ++u) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) x[u][r] = (__builtin_fmaf(x[u][r], c, shift[u]) - base) / c;
+          for (int r = 0; r < 16; ++r) x[u][r] = (__builtin_fmaf(x[u][r], c, shift[u]) - base + kLift<T>) / c;
           shift[u] = 0.f;
         }
-        base = 0.f;
+        base = kLift<T>;
       }
     }
 #pragma unroll
     for (int u = 0; u < KT / 32; ++u) {
-      const float off = shift[u] - base;
+      const float off = shift[u] - base + kLift<T>;
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][r], c, off));
 #pragma unroll
@@ -543,7 +549,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams 
   const float f = any ? 1.f / sum : 0.f;
   store_turned<T, D>(mine, (T*)p.out + (s.begin + i0) * hd + (long long)head * D, hd, acc, f, len - i0);
   if (p.rest) store_turned<T, D, true>(mine, (T*)p.rest + (s.begin + i0) * hd + (long long)head * D, hd, acc, f, len - i0);
-  if (p.lse && lane < 32 && i0 + l < len) p.lse[(long long)head * p.total + s.begin + i0 + l] = any ? m + __log2f(sum) : INFINITY;
+  if (p.lse && lane < 32 && i0 + l < len) p.lse[(long long)head * p.total + s.begin + i0 + l] = any ? m + (__log2f(sum) - kLift<T>) : INFINITY;
 }
 
 // A 32x32 tile's sums by distance, keys in the registers.  Register r's key is row(r) and a lane's query 16 b + c, so shifting the 16
@@ -783,7 +789,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_any_kernel(const AttnPa
   const float* lse = p.lse + (long long)head * p.total + s.begin;
   const float* delta = p.delta + (long long)head * p.total + s.begin;
   const float* fix = p.fix + (long long)head * p.total + s.begin;
-  const float lift = ds_lift<T>(p, head, s.b);
+  const float lift = ds_lift<T>(p, head, s.b), down = lift * kUnlift<T>;
   const float c = p.scale * kLog2e;
   f32x16 ak[DP / 32] = {}, av[DP / 32] = {};
   for (int i0 = 0; i0 < len; i0 += 32) {
@@ -804,16 +810,16 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_any_kernel(const AttnPa
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int row = (r & 3) + 8 * (r >> 2) + 4 * half;
-      t[r] = __builtin_amdgcn_exp2f(t[r] - sl[row] - sf[row]);
+      t[r] = __builtin_amdgcn_exp2f(t[r] - sl[row] - sf[row] + kLift<T>);
       ds[r] = t[r] == 0.f ? 0.f : t[r] * (dp[r] - sd[row]);
     }
     trans_times<T, DP>(av, sgt, t);
-    if (lift != 1.f) ds *= lift;
+    if (down != 1.f) ds *= down;
     trans_times<T, DP>(ak, sqt, ds);
   }
   if (j >= len) return;
   store_cols<T, DP>((T*)p.dk + (s.begin + j) * p.gld_t + head * p.gld_h, ak, p.scale / lift, p.d, p.vec);
-  store_cols<T, DP>((T*)p.dv + (s.begin + j) * p.gld_t + head * p.gld_h, av, 1.f, p.d, p.vec);
+  store_cols<T, DP>((T*)p.dv + (s.begin + j) * p.gld_t + head * p.gld_h, av, kUnlift<T>, p.d, p.vec);
 }
 
 // ---- backward, whole 16-byte pieces and head widths of 32, 64 and 128 -------------------------------------------------------
@@ -1084,7 +1090,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
 #pragma unroll
     for (int x = 0; x < D / (2 * V); ++x) { fk[x] = *(const vec*)(k + x * 2 * V); fv[x] = *(const vec*)(v + x * 2 * V); }
   }
-  const float lift = ds_lift<T>(p, head, s.b);
+  const float lift = ds_lift<T>(p, head, s.b), down = lift * kUnlift<T>;
   const float c = p.scale * kLog2e;
   make_start_line<T>(line, p, head, c, len + QT);
   const float* mid = line + start_at(p.reach, l - 4 * half);        // mid[e0 - row]: column l is the key, the rows are queries
@@ -1117,9 +1123,11 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int row = u * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
-          x[r] = (__builtin_fmaf(x[r], c, shift) - stat[t & 1][2][row] - stat[t & 1][3][row]) / c;
+          x[r] = (__builtin_fmaf(x[r], c, shift) - stat[t & 1][2][row] - stat[t & 1][3][row] + kLift<T>) / c;
         }
         shift = 0.f;
+      } else {
+        shift += kLift<T>;
       }
 #pragma unroll
       for (int y = 0; y < D / (2 * V); ++y) Elem<T>::mma(R::along(sg, u * 32, y), fv[y], dp);
@@ -1134,7 +1142,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
         }
       }
       add_across<T, D>(av, sg, u * 32, x);
-      if (lift != 1.f) dp *= lift;
+      if (down != 1.f) dp *= down;
       add_across<T, D>(ak, sq, u * 32, dp);
     }
   }
@@ -1143,7 +1151,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
   // 32 rows at a time through the wave's part of LDS
   T* mine = &buf[0][0][0] + wave * (32 * D);
   store_turned<T, D>(mine, (T*)p.dk + (s.begin + j0) * p.gld_t + head * p.gld_h, p.gld_t, ak, p.scale / lift, len - j0);
-  store_turned<T, D>(mine, (T*)p.dv + (s.begin + j0) * p.gld_t + head * p.gld_h, p.gld_t, av, 1.f, len - j0);
+  store_turned<T, D>(mine, (T*)p.dv + (s.begin + j0) * p.gld_t + head * p.gld_h, p.gld_t, av, kUnlift<T>, len - j0);
 }
 
 // dtable[t][h] = the slots' parts in order, in 64 bits: block = one head and bucket
