@@ -62,7 +62,7 @@ def main():
                 e = MPNetEmbedder(d, device="cuda:0", autocast=amp, engine=engine)
                 some = e.embed_device(sets["2048_texts_5_to_32"][0][:64])
                 plain = some if plain is None else plain
-                line = {"precision": amp or "fp32", "engine": engine, "error": float((some - plain).norm(dim=1).mean())}
+                line = {"precision": amp or "fp32", "engine": engine, "error": float(f"{float((some - plain).norm(dim=1).mean()):.3g}")}
                 line.update({n: round(ms(lambda: e.embed_device(texts), k), 3) for n, (texts, k) in sets.items()})
                 lines.append(line)
                 print(json.dumps(line), flush=True)
