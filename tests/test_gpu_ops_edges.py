@@ -312,3 +312,16 @@ def test_attention_small_probabilities_keep_their_bits_in_fp16(ops, d, small):
     part = (n - 1) * p * 2.0 ** 14
     assert ((out.detach().cpu().double() - part).abs() <= rel * part + 2.0 ** -25).all()
     assert ((dv[keep] - p * 2.0 ** 14).abs() <= rel * p * 2.0 ** 14 + 2.0 ** -25).all()
+
+
+def test_an_error_is_reported_once(ops, hip_lib):
+    """A call refused by the runtime leaves nothing behind for the next call, or for torch's next kernel."""
+    x, w = torch.ones(5, 8, device="cuda"), torch.ones(3, 8, device="cuda")
+    want, out = ops.linear(x, w), torch.empty(5, 3, device="cuda")
+    off = offsets_of([5])
+    for call in (lambda: hip_lib.vdb_op_linear_dev(99, 0, x.data_ptr(), 8, w.data_ptr(), 8, None, None, 0, out.data_ptr(), 3, None, 5, 3, 8, 0, None, 0, None),
+                 lambda: hip_lib.vdb_op_mean_pool_dev(99, 0, x.data_ptr(), 8, off.data_ptr(), 1, 5, 8, 1, out.data_ptr(), None, None)):
+        assert call() == -2 and b"device" in hip_lib.vdb_last_error(None)
+        assert torch.equal(ops.linear(x, w), want)
+        assert call() == -2
+        assert (torch.ones(4, device="cuda") + 1).sum().item() == 8

@@ -19,6 +19,7 @@ int bad(int code, const char* what) {
 int hip_fail(const char* where, hipError_t e) {
   char msg[256];
   snprintf(msg, sizeof msg, "%s: %s", where, hipGetErrorString(e));
+  (void)hipGetLastError();     // reported here: the next launch on this thread, whoever's, must not find it again
   return bad(e == hipErrorOutOfMemory ? VDB_ERR_MEMORY : VDB_ERR_DEVICE, msg);
 }
 #define NEED(cond, what) do { if (!(cond)) return bad(VDB_ERR_ARG, what); } while (0)
