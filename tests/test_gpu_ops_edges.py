@@ -325,3 +325,19 @@ def test_an_error_is_reported_once(ops, hip_lib):
         assert torch.equal(ops.linear(x, w), want)
         assert call() == -2
         assert (torch.ones(4, device="cuda") + 1).sum().item() == 8
+
+
+def test_a_stores_failed_reservation_is_reported_once(ops, hip_lib):
+    """Rows that no GPU holds are refused by the allocator, and the operators' and torch's next calls do not hear of it."""
+    from vectordb_amd import VdbError
+    from vectordb_amd.index import FlatIndex
+    x, w = torch.ones(5, 8, device="cuda"), torch.ones(3, 8, device="cuda")
+    want = ops.linear(x, w)
+    idx = FlatIndex(4096)
+    for _ in range(2):
+        with pytest.raises(VdbError):
+            idx.reserve(2 ** 31 - 4096)              # 35 TB
+        assert torch.equal(ops.linear(x, w), want)
+        with pytest.raises(VdbError):
+            idx.reserve(2 ** 31 - 4096)
+        assert (torch.ones(4, device="cuda") + 1).sum().item() == 8

@@ -180,6 +180,7 @@ namespace {
 
 int fail(vdb_t* h, int code, const std::string& msg) {
   if (h) h->err = msg; else g_err = msg;
+  if (code == VDB_ERR_DEVICE || code == VDB_ERR_MEMORY) (void)hipGetLastError();   // reported here: the next launch on this thread must not find it again
   return code;
 }
 
