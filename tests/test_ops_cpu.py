@@ -177,3 +177,12 @@ def test_tracers_are_refused():
                 call(arg)
         with FlopCounterMode(display=False), pytest.raises(ValueError, match="GPU"):
             call(arg)
+
+
+def test_an_optional_tensor_without_memory_is_not_an_absent_one():
+    """A bias whose storage was freed has a null address, which the C ABI takes for none."""
+    t = torch.ones(3)
+    assert ops._ptr(None) is None and ops._ptr(t) == t.data_ptr() and not ops._ptr(torch.ones(0))
+    t.untyped_storage().resize_(0)
+    with pytest.raises(ValueError, match="no memory"):
+        ops._ptr(t)

@@ -64,7 +64,13 @@ def _scratch(n: int, like: torch.Tensor) -> Optional[torch.Tensor]:
 
 
 def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+    """An optional tensor's address.  One without memory (a freed storage, a wrapper around other tensors) is not an absent one."""
+    if t is None:
+        return None
+    p = t.data_ptr()
+    if not p and t.numel():
+        raise ValueError(f"a tensor of shape {tuple(t.shape)} has no memory of its own")
+    return p
 
 
 _is_tracing, _modes, _key_included = torch._C._is_tracing, torch._C._len_torch_dispatch_stack, torch._C._dispatch_tls_is_dispatch_key_included
