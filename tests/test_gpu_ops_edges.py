@@ -341,3 +341,30 @@ def test_a_stores_failed_reservation_is_reported_once(ops, hip_lib):
         with pytest.raises(VdbError):
             idx.reserve(2 ** 31 - 4096)
         assert (torch.ones(4, device="cuda") + 1).sum().item() == 8
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [24, 64])
+def test_attention_of_broadcast_inputs(ops, dtype, d):
+    """One bias column for all heads, one head, one row or one of q, k and v for all: the same outputs as from copies, and the copies' gradients
+    summed."""
+    t, n, heads = DT[dtype], 70, 4
+    g = torch.Generator().manual_seed(d)
+    off = offsets_of([50, 20])
+    dout = rnd(g, n, heads, d, dtype=t).cuda()
+    shapes = {"heads": (n, 3, 1, d), "rows": (1, 3, heads, d), "the three": (n, 1, heads, d)}
+    column = rnd(g, 32, 1, dtype=t).cuda()
+    for name, shape in shapes.items():
+        small = rnd(g, *shape, dtype=t).cuda()
+        one, col = small.clone().requires_grad_(), column.clone().requires_grad_()
+        out = ops.bucketed_attention(one.expand(n, 3, heads, d), col.expand(32, heads), off)
+        got = torch.autograd.grad(out, [one, col], dout)
+        full, table = small.expand(n, 3, heads, d).contiguous().requires_grad_(), column.expand(32, heads).contiguous().requires_grad_()
+        want = ops.bucketed_attention(full, table, off)
+        assert torch.equal(out, want), name
+        whole = torch.autograd.grad(want, [full, table], dout)
+        dims = [i for i, s in enumerate(shape) if s == 1]
+        for a, b, axes in ((got[0], whole[0], dims), (got[1], whole[1], [1])):
+            exact = b.double().sum(axes, keepdim=True)
+            # autograd's sum over the copies, rounded to the type at each of at most n steps
+            assert ((a.double() - exact).abs() <= 2 * n * ref.half_step(t) * b.double().abs().sum(axes, keepdim=True) + 1e-30).all(), name
