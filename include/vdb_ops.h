@@ -57,8 +57,8 @@ int vdb_op_linear_backward_dev(int device, int dtype, const void* dy, int64_t ld
  * bucket(e), with half = n_buckets/2, near = half/2, n = |e|: n below near, else near + the number of i in 1..half-near-1
  * with n >= near (max_distance/near)^(i/(half-near)) (compared in whole numbers); + half where e > 0.  This is the
  * bidirectional bucketing of the reference's embedding model (32 buckets, max_distance 128).
- * A bias of -inf forbids its distances; a row that is left nothing gives zeros, one whose biases are all the same great finite number an even
- * softmax.  Scales outside [1e-18, 1e18] take the general kernels.
+ * A bias of -inf forbids its distances; a row that is left nothing gives zeros, one whose biases are all the same finite number, so great
+ * that the scores vanish beside it in 32 bits, an even softmax.  Scales outside [1e-18, 1e18] take the general kernels.
  * q, k, v: token stride ld_t, head stride ld_h, dense head rows of head_dim.  out: dense [total][heads][head_dim].
  * Kept for the backward pass, each may be NULL: lse fp32 [heads][total], log2 of the softmax denominators; rest, of out's type and
  * shape, what the rounding of out left (16-bit types: the gradients need rowsum(dout out) closer than that rounding). */
