@@ -368,3 +368,30 @@ def test_attention_of_broadcast_inputs(ops, dtype, d):
             exact = b.double().sum(axes, keepdim=True)
             # autograd's sum over the copies, rounded to the type at each of at most n steps
             assert ((a.double() - exact).abs() <= 2 * n * ref.half_step(t) * b.double().abs().sum(axes, keepdim=True) + 1e-30).all(), name
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [24, 32, 64, 128])
+def test_attention_great_scores_beside_greater_biases(ops, dtype, d):
+    """Biases of 1e12 and scores of 1e10: steps of 1e5 in 32 bits, which different orders of the same sums do not share.  Forward and in v's
+    gradient a row is still its greatest score's alone."""
+    t, n = DT[dtype], 150
+    g = torch.Generator().manual_seed(d)
+    qkv, dout = rnd(g, n, 3, 1, d, dtype=t), rnd(g, n, 1, d, dtype=t)
+    qkv[:, :2] *= 1e5
+    table = torch.full((32, 1), 1e12).to(t)
+    q, k, v = qkv[:, :, 0].double().unbind(1)
+    s = d ** -0.5 * (q @ k.t())
+    top = s.topk(2, 1)
+    clear = top.values[:, 0] - top.values[:, 1] > 16 * 1e12 * ref.E * (d + 4)      # d roundings of sums of 1e12, and both sides' few more
+    assert clear.sum() > n // 2
+    dout[~clear] = 0
+    lq = qkv.cuda().requires_grad_()
+    out = ops.bucketed_attention(lq, table.cuda(), offsets_of([n]))
+    dqkv, = torch.autograd.grad(out, [lq], dout.cuda())
+    assert torch.isfinite(out).all() and torch.isfinite(dqkv).all()
+    best = top.indices[:, 0]
+    assert torch.equal(out.detach().cpu()[clear, 0], qkv[best[clear], 2, 0])
+    want = torch.zeros(n, d, dtype=torch.float64).index_add_(0, best, dout[:, 0].double())
+    size = torch.zeros(n, d, dtype=torch.float64).index_add_(0, best, dout[:, 0].double().abs())
+    hold([dqkv[:, 2, 0]], [(want, (n + 16) * ref.E * size + ref.half_step(t) * want.abs() + 2.0 ** -120)], dtype)

@@ -71,10 +71,24 @@ __device__ __forceinline__ void make_line(float* line, const AttnParams& p, int 
 // - s is rounded before m is taken away.  Fused, scale x - m keeps the product's exact tail, and half a step of a number like 1e38 is far
 //   beyond any exponent.
 // - The kept lse = m + log2(sum) has no room for log2(sum) there (at the type's lowest value p would be 1 instead of 1 / len): the backward
-//   pass sums the row's exp2(s - lse) once more and takes log2 of that away too (`fix`, 0 for other rows).
+//   pass sums the row's exp2(s - lse) once more and takes log2 of that away too (`fix`, 0 for other rows).  It sums them from their own
+//   greatest: s may have come out some steps of 1e12 apart from the forward pass' where other kernels made that (fp32 heads of 128).
 // The tiled kernels do so in a branch ahead of the exponentials that turns a tile's x into (s - m) / c, so that what every tile runs
 // through stays as it is: with a second form of the exponentials in the loop, 16 x 384 tokens in fp32 took 107 us instead of 85.
 __device__ __forceinline__ bool is_great(float x) { return fabsf(x) > 1024.f && fabsf(x) < INFINITY; }
+
+// log2 of a row's sum of exp2(x), one x after the other; half a row a lane
+struct RowSum {
+  float top = -INFINITY, sum = 0.f;
+  __device__ __forceinline__ void add(float x) {
+    if (x > top) { sum = sum * __builtin_amdgcn_exp2f(top - x) + 1.f; top = x; }
+    else if (x != -INFINITY) sum += __builtin_amdgcn_exp2f(x - top);       // NaN stays
+  }
+  __device__ __forceinline__ float log() {
+    const float top2 = __shfl_xor(top, 32, 64), sum2 = __shfl_xor(sum, 32, 64), m = fmaxf(top, top2);
+    return m + log2f((sum == 0.f ? 0.f : sum * __builtin_amdgcn_exp2f(top - m)) + (sum2 == 0.f ? 0.f : sum2 * __builtin_amdgcn_exp2f(top2 - m)));
+  }
+};
 
 // fp16 operands: p <= 1 would lose bits below 2^-14 and vanish below 2^-25 (beside a key of nearly all the weight, or 1 / len of a text of
 // 20 thousand tokens); as 2^15 p it keeps them down to 2^-29.  The sums carry the factor too, dv and ds are freed of it.
@@ -208,7 +222,7 @@ __device__ __forceinline__ void add_bias(f32x16& s, float c, const float* line, 
   if (tile_is_far(e0, reach)) {
     const float b = line[e0 > 0 ? 2 * reach : 0];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = s[r] * c + b;
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], c, b);      // rounded once in every kernel: see is_great
     return;
   }
 #pragma unroll
@@ -216,7 +230,7 @@ __device__ __forceinline__ void add_bias(f32x16& s, float c, const float* line, 
     const int row = (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5), col = lane & 31;
     int e = e0 + (KEYS_IN_ROWS ? row - col : col - row);
     e = e > reach ? reach : e < -reach ? -reach : e;
-    s[r] = s[r] * c + line[reach + e];
+    s[r] = __builtin_fmaf(s[r], c, line[reach + e]);
   }
 }
 
@@ -704,7 +718,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_any_kernel(const AttnPar
   const float c = p.scale * kLog2e;
   float fix = 0.f;
   if (__builtin_amdgcn_readfirstlane(__syncthreads_or(is_great(lse)))) {
-    float sum = 0.f;
+    RowSum row;
     for (int j0 = 0; j0 < len; j0 += 32) {
       __syncthreads();
       stage_rows<T, DP, 32, true, false>(sk, nullptr, kb + j0 * p.ld_t, p.ld_t, len - j0, p.d, p.vec, NW * 64);
@@ -712,10 +726,10 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_any_kernel(const AttnPar
       f32x16 t = rows_times<T, DP>(sk, fq);
       add_bias<true>(t, c, line, reach, j0 - i0);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) if (j0 + (r & 3) + 8 * (r >> 2) + 4 * half < len) sum += __builtin_amdgcn_exp2f(t[r] - lse);
+      for (int r = 0; r < 16; ++r) if (j0 + (r & 3) + 8 * (r >> 2) + 4 * half < len) row.add(t[r] - lse);
     }
-    sum += __shfl_xor(sum, 32, 64);
-    if (is_great(lse)) fix = log2f(sum);
+    const float all = row.log();
+    if (is_great(lse)) fix = all;
   }
   if (lane < 32 && i < len) p.fix[(long long)head * p.total + s.begin + i] = fix;
   float below = 0.f, above = 0.f;
@@ -958,7 +972,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
   float fix = 0.f;
   const bool great = __builtin_amdgcn_readfirstlane(__syncthreads_or(is_great(lse)));
   if (great) {
-    float sum = 0.f;
+    RowSum all;
     for (int t = 0; t < tiles; ++t) {
       wait_loads<0>();
       __syncthreads();
@@ -972,11 +986,11 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
         const float bias = c * scores<T, D, R, 1>(x, buf[t & 1][0], u * 32, fq, e0, p, line, mid + e0);
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (j0 + (r & 3) + 8 * (r >> 2) + 4 * half < len) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], c, bias) + from);
+          if (j0 + (r & 3) + 8 * (r >> 2) + 4 * half < len) all.add(__builtin_fmaf(x[r], c, bias) + from);
       }
     }
-    sum += __shfl_xor(sum, 32, 64);
-    if (is_great(lse)) fix = log2f(sum);
+    const float log = all.log();
+    if (is_great(lse)) fix = log;
     __syncthreads();                 // the last tile is read: its place may be loaded again
     issue(0);
   }
