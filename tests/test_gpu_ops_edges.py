@@ -395,3 +395,25 @@ def test_attention_great_scores_beside_greater_biases(ops, dtype, d):
     want = torch.zeros(n, d, dtype=torch.float64).index_add_(0, best, dout[:, 0].double())
     size = torch.zeros(n, d, dtype=torch.float64).index_add_(0, best, dout[:, 0].double().abs())
     hold([dqkv[:, 2, 0]], [(want, (n + 16) * ref.E * size + ref.half_step(t) * want.abs() + 2.0 ** -120)], dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [24, 32, 64, 128])
+def test_attention_rows_sum_to_one_beside_great_biases(ops, dtype, d):
+    """Biases of -1e20 and scores of 1e14: in 32 bits some of a row's greatest scores are one number, and share the row.  Whatever p is there,
+    with v = 1 an output is 1, and each row hands all of its gradient on to v."""
+    t, n = DT[dtype], 52
+    ones = torch.ones(n, 1, d, dtype=t)
+    for seed in range(40):
+        g = torch.Generator().manual_seed(seed)
+        qkv = rnd(g, n, 3, 1, d, dtype=t)
+        qkv[:, :2] *= 1e8
+        qkv[:, 2] = 1
+        lq = qkv.cuda().requires_grad_()
+        out = ops.bucketed_attention(lq, torch.full((32, 1), -1e20, dtype=t, device="cuda"), offsets_of([n]), scale=1e-3)
+        dqkv, = torch.autograd.grad(out, [lq], ones.cuda())
+        # halves, thirds and the like, rounded to the type; sums of 52 rows
+        u = ref.half_step(t)
+        assert ((out.detach().float() - 1).abs() <= 4 * u + 64 * ref.E).all()
+        assert ((dqkv[:, 2].double().sum(0) - n).abs() <= n * (4 * u + 64 * ref.E)).all()
+        assert torch.isfinite(dqkv).all()

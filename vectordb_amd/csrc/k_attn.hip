@@ -103,7 +103,7 @@ hipError_t run_dp(const AttnParams& p, const AttnArgs& a, bool back) {
 template <typename T>
 hipError_t run_t(const AttnArgs& a, bool back) {
   AttnParams p = params(a, sizeof(T));
-  p.delta = a.delta; p.fix = a.fix; p.part = a.part; p.peak = (const unsigned*)a.gscale; p.order = (const i32x4*)a.order;
+  p.delta = a.delta; p.from = a.from; p.fix = a.fix; p.part = a.part; p.peak = (const unsigned*)a.gscale; p.order = (const i32x4*)a.order;
   if (back) {
     const unsigned grid = (unsigned)(n_slots(p.total, p.n_seqs, 32) * p.heads);
     if (a.gscale) {
@@ -128,12 +128,14 @@ hipError_t launch_attention(int dtype, const AttnArgs& a) {
 
 int64_t attention_backward_workspace(int dtype, int64_t n_seqs, int64_t total, int heads, int d, int n_buckets) {
   const int64_t slots = n_slots(total, n_seqs, 32 * tile_waves(dtype, d, true, n_seqs, total));
-  return 2 * pad256(total * heads * 4) + (dtype == 2 ? pad256(2 * n_seqs * heads * 4) : 0) + pad256(slots * heads * n_buckets * 4) +
+  return 3 * pad256(total * heads * 4) + (dtype == 2 ? pad256(2 * n_seqs * heads * 4) : 0) + pad256(slots * heads * n_buckets * 4) +
          (by_length(n_seqs, total, slots, heads) ? pad256(slots * 16) : 0);
 }
 
 hipError_t launch_attention_backward(int dtype, AttnArgs a, char* ws) {
   a.delta = (float*)ws;
+  ws += pad256(a.total * a.heads * 4);
+  a.from = (float*)ws;
   ws += pad256(a.total * a.heads * 4);
   a.fix = (float*)ws;
   ws += pad256(a.total * a.heads * 4);

@@ -23,7 +23,7 @@ struct AttnParams {
   int heads, d; float scale;
   void* out; void* rest; float* lse;
   const void* dout; void *dq, *dk, *dv; long long gld_t, gld_h;
-  float* delta; float* fix; const unsigned* peak; float* part;   // peak: [2][heads][n_seqs] largest |dout| and |v| (fp16 only)
+  float* delta; float* from; float* fix; const unsigned* peak; float* part;   // peak: [2][heads][n_seqs] largest |dout| and |v| (fp16 only)
   const i32x4* order;   // the tiled backward kernels' places, longest sequences first, or nullptr
   int vec;        // q, k, v, out, dout, gradients: 16-byte rows
   int reach;      // R
@@ -71,22 +71,24 @@ __device__ __forceinline__ void make_line(float* line, const AttnParams& p, int 
 // - s is rounded before m is taken away.  Fused, scale x - m keeps the product's exact tail, and half a step of a number like 1e38 is far
 //   beyond any exponent.
 // - The kept lse = m + log2(sum) has no room for log2(sum) there (at the type's lowest value p would be 1 instead of 1 / len): the backward
-//   pass sums the row's exp2(s - lse) once more and takes log2 of that away too (`fix`, 0 for other rows).  It sums them from their own
-//   greatest: s may have come out some steps of 1e12 apart from the forward pass' where other kernels made that (fp32 heads of 128).
+//   pass takes such rows' greatest score and sum once more, and keeps the two apart (`from` and `fix`; lse and 0 for other rows).  It takes
+//   both from its own scores: some steps of 1e12 may lie between those and the forward pass' where another kernel made that (fp32
+//   heads of 128).
 // The tiled kernels do so in a branch ahead of the exponentials that turns a tile's x into (s - m) / c, so that what every tile runs
 // through stays as it is: with a second form of the exponentials in the loop, 16 x 384 tokens in fp32 took 107 us instead of 85.
 __device__ __forceinline__ bool is_great(float x) { return fabsf(x) > 1024.f && fabsf(x) < INFINITY; }
 
-// log2 of a row's sum of exp2(x), one x after the other; half a row a lane
+// A row's greatest score and log2 of its sum of exp2(s - greatest), one s after the other; half a row a lane
 struct RowSum {
   float top = -INFINITY, sum = 0.f;
-  __device__ __forceinline__ void add(float x) {
-    if (x > top) { sum = sum * __builtin_amdgcn_exp2f(top - x) + 1.f; top = x; }
-    else if (x != -INFINITY) sum += __builtin_amdgcn_exp2f(x - top);       // NaN stays
+  __device__ __forceinline__ void add(float s) {
+    if (s > top) { sum = sum * __builtin_amdgcn_exp2f(top - s) + 1.f; top = s; }
+    else if (s != -INFINITY) sum += __builtin_amdgcn_exp2f(s - top);       // NaN stays
   }
-  __device__ __forceinline__ float log() {
+  __device__ __forceinline__ void join() {
     const float top2 = __shfl_xor(top, 32, 64), sum2 = __shfl_xor(sum, 32, 64), m = fmaxf(top, top2);
-    return m + log2f((sum == 0.f ? 0.f : sum * __builtin_amdgcn_exp2f(top - m)) + (sum2 == 0.f ? 0.f : sum2 * __builtin_amdgcn_exp2f(top2 - m)));
+    sum = (sum == 0.f ? 0.f : sum * __builtin_amdgcn_exp2f(top - m)) + (sum2 == 0.f ? 0.f : sum2 * __builtin_amdgcn_exp2f(top2 - m));
+    top = m;
   }
 };
 
@@ -712,7 +714,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_any_kernel(const AttnPar
   typename Elem<T>::vec fq[DP / (2 * V)], fg[DP / (2 * V)];
   load_row_frags<T, DP>(fq, (const T*)p.q + (s.begin + i) * p.ld_t + head * p.ld_h, i < len, p.d, p.vec);
   load_row_frags<T, DP>(fg, (const T*)p.dout + (s.begin + i) * hd + (long long)head * p.d, i < len, p.d, p.vec);
-  const float lse = i < len ? p.lse[(long long)head * p.total + s.begin + i] : INFINITY;
+  float lse = i < len ? p.lse[(long long)head * p.total + s.begin + i] : INFINITY;
   const float delta = i < len ? p.delta[(long long)head * p.total + s.begin + i] : 0.f;
   const float lift = ds_lift<T>(p, head, s.b);
   const float c = p.scale * kLog2e;
@@ -726,12 +728,12 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_any_kernel(const AttnPar
       f32x16 t = rows_times<T, DP>(sk, fq);
       add_bias<true>(t, c, line, reach, j0 - i0);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) if (j0 + (r & 3) + 8 * (r >> 2) + 4 * half < len) row.add(t[r] - lse);
+      for (int r = 0; r < 16; ++r) if (j0 + (r & 3) + 8 * (r >> 2) + 4 * half < len) row.add(t[r]);
     }
-    const float all = row.log();
-    if (is_great(lse)) fix = all;
+    row.join();
+    if (is_great(lse)) { lse = row.top; fix = log2f(row.sum); }
   }
-  if (lane < 32 && i < len) p.fix[(long long)head * p.total + s.begin + i] = fix;
+  if (lane < 32 && i < len) { p.from[(long long)head * p.total + s.begin + i] = lse; p.fix[(long long)head * p.total + s.begin + i] = fix; }
   float below = 0.f, above = 0.f;
   f32x16 acc[DP / 32] = {};
   for (int j0 = 0; j0 < len; j0 += 32) {
@@ -800,7 +802,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_any_kernel(const AttnPa
   load_row_frags<T, DP>(fv, (const T*)p.v + (s.begin + j) * p.ld_t + head * p.ld_h, j < len, p.d, p.vec);
   const T* qb = (const T*)p.q + s.begin * p.ld_t + head * p.ld_h;
   const T* gb = (const T*)p.dout + s.begin * hd + (long long)head * p.d;
-  const float* lse = p.lse + (long long)head * p.total + s.begin;
+  const float* lse = p.from + (long long)head * p.total + s.begin;
   const float* delta = p.delta + (long long)head * p.total + s.begin;
   const float* fix = p.fix + (long long)head * p.total + s.begin;
   const float lift = ds_lift<T>(p, head, s.b), down = lift * kUnlift<T>;
@@ -942,7 +944,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
     for (int x = 0; x < D / (2 * V); ++x) { fq[x] = *(const vec*)(q + x * 2 * V); fg[x] = *(const vec*)(g + x * 2 * V); }
   }
   const long long row = (long long)head * p.total + s.begin + i;
-  const float lse = i0 + l < len ? p.lse[row] : INFINITY;
+  float lse = i0 + l < len ? p.lse[row] : INFINITY;
   float delta = 0.f;                 // dout . out, for this kernel and, through memory, for dk
   {
     const T* o = (const T*)p.out + (s.begin + i) * hd + (long long)head * D + half * V;
@@ -966,8 +968,8 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
   float* mine = hist + (wave * 2 + half) * span;
 #pragma unroll
   for (int x = 0; x < D / (2 * V); ++x) { settle(fq[x]); settle(fg[x]); }
-  float from = -lse, less = delta;
-  settle(from);
+  float less = delta;
+  settle(lse);
   settle(less);
   float fix = 0.f;
   const bool great = __builtin_amdgcn_readfirstlane(__syncthreads_or(is_great(lse)));
@@ -986,15 +988,16 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
         const float bias = c * scores<T, D, R, 1>(x, buf[t & 1][0], u * 32, fq, e0, p, line, mid + e0);
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (j0 + (r & 3) + 8 * (r >> 2) + 4 * half < len) all.add(__builtin_fmaf(x[r], c, bias) + from);
+          if (j0 + (r & 3) + 8 * (r >> 2) + 4 * half < len) all.add(__builtin_fmaf(x[r], c, bias));
       }
     }
-    const float log = all.log();
-    if (is_great(lse)) fix = log;
+    all.join();
+    if (is_great(lse)) { lse = all.top; fix = log2f(all.sum); }
     __syncthreads();                 // the last tile is read: its place may be loaded again
     issue(0);
   }
-  if (lane < 32 && i0 + l < len) p.fix[row] = fix;
+  if (lane < 32 && i0 + l < len) { p.from[row] = lse; p.fix[row] = fix; }
+  const float from = -lse;
   float below = 0.f, above = 0.f;
   f32x16 acc[D / 32] = {};
   for (int t = 0; t < tiles; ++t) {
@@ -1080,7 +1083,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
   const long long hd = (long long)p.heads * D;
   const T* qb = (const T*)p.q + s.begin * p.ld_t + head * p.ld_h;
   const T* gb = (const T*)p.dout + s.begin * hd + (long long)head * D;
-  const float* lse = p.lse + (long long)head * p.total + s.begin;
+  const float* lse = p.from + (long long)head * p.total + s.begin;
   const float* delta = p.delta + (long long)head * p.total + s.begin;
   const float* fix = p.fix + (long long)head * p.total + s.begin;
   float next_lse = 0.f, next_delta = 0.f, next_fix = 0.f;    // thread x < QT, the first wave: of query x of the tile under way
@@ -1113,7 +1116,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
   f32x16 ak[D / 32] = {}, av[D / 32] = {};
   for (int t = 0; t < tiles; ++t) {
     if (threadIdx.x < QT) {
-      const bool any = __any(is_great(next_lse));
+      const bool any = __any(is_great(next_lse) || next_fix != 0.f);
       stat[t & 1][0][threadIdx.x] = any ? 0.f : next_lse;
       stat[t & 1][1][threadIdx.x] = next_delta;
       stat[t & 1][2][threadIdx.x] = next_lse;

@@ -42,7 +42,7 @@ struct AttnArgs {
   void* out; void* rest; float* lse;     // rest: what the rounding of out left, or nullptr
   // backward
   const void* dout; void *dq, *dk, *dv; int64_t gld_t, gld_h; void* dtable;
-  float* delta; float* fix; float* gscale; float* part; void* order;    // workspace pieces
+  float* delta; float* from; float* fix; float* gscale; float* part; void* order;    // workspace pieces
   hipStream_t st;
 };
 hipError_t launch_attention(int dtype, const AttnArgs& a);
