@@ -417,3 +417,27 @@ def test_attention_rows_sum_to_one_beside_great_biases(ops, dtype, d):
         assert ((out.detach().float() - 1).abs() <= 4 * u + 64 * ref.E).all()
         assert ((dqkv[:, 2].double().sum(0) - n).abs() <= n * (4 * u + 64 * ref.E)).all()
         assert torch.isfinite(dqkv).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [24, 32, 64, 128])
+def test_attention_scores_are_the_same_numbers_forward_and_back(ops, dtype, d):
+    """Texts of one token, whose score is a small difference of a great bias and a great product: p is 1 both ways only where both passes make
+    that difference in the same order."""
+    t, n = DT[dtype], 64
+    scale, bias = (1e-3, -1e4) if dtype != "f16" else (1.0, -1e4)
+    g = torch.Generator().manual_seed(d)
+    qkv, dout = rnd(g, n, 3, 1, d, dtype=t), rnd(g, n, 1, d, dtype=t)
+    qkv[:, 0] = (1e4 / scale / d) ** 0.5                      # q.k close to 1e4 / scale
+    qkv[:, 1] = (qkv[:, 0].double() * (1 + 0.05 * torch.randn(n, 1, d, generator=g).double())).to(t)
+    leaf = qkv.cuda().requires_grad_()
+    out = ops.bucketed_attention(leaf, torch.full((32, 1), bias, dtype=t, device="cuda"), offsets_of([1] * n), scale=scale)
+    dqkv, = torch.autograd.grad(out, [leaf], dout.cuda())
+    s = (scale * (qkv[:, 0, 0].double() * qkv[:, 1, 0].double()).sum(1) + float(torch.tensor(bias, dtype=t))).abs().max()
+    # lse is rounded (E |s| log2(e) ln 2 in p), p to the type, the result to the type
+    rel = 2 * float(s) * ref.E + 8 * ref.E + 2 * ref.half_step(t)
+    # p is not 1 to the last bit in fp32 (the score's product is exact inside the exponent, its maximum rounded): out = (p v) (1 / p), three
+    # roundings of E and their products
+    v = qkv[:, 2, 0].double()
+    assert ((out.detach().cpu()[:, 0].double() - v).abs() <= 4 * ref.E * v.abs()).all()
+    assert ((dqkv[:, 2].cpu().double() - dout.double()).abs() <= rel * dout.double().abs() + 2.0 ** -25).all()

@@ -54,8 +54,7 @@ __device__ __forceinline__ float start_value(float b, float scale, float c) {
   return __builtin_isinf(b) ? b : x > most ? most : x < -most ? -most : x;
 }
 
-// line[R + e] = bias(e) * log2(e) for |e| <= R: by the same steps as in the tiled kernels where they may have made the other pass (fp32
-// heads of 128), so that great biases come out as the same numbers in both.
+// line[R + e] for |e| <= R: what a tile's sums start from, as in the tiled kernels (scores_any); bias(e) * log2(e) where the scale is not even
 template <typename T>
 __device__ __forceinline__ void make_line(float* line, const AttnParams& p, int head) {
   const float c = p.scale * kLog2e;
@@ -63,7 +62,7 @@ __device__ __forceinline__ void make_line(float* line, const AttnParams& p, int 
     const float b = (float)((const T*)p.table)[(long long)bucket_of(p.bk, t - p.reach) * p.heads + head];
     float x = b * kLog2e;
     if (__builtin_isinf(x) && !__builtin_isinf(b)) x = b < 0.f ? -3.4028234e38f : 3.4028234e38f;
-    line[t] = even_scale(p.scale) ? start_value(b, p.scale, c) * c : x;
+    line[t] = even_scale(p.scale) ? start_value(b, p.scale, c) : x;
   }
 }
 
@@ -139,12 +138,11 @@ __device__ __forceinline__ void load_row_frags(typename Elem<T>::vec (&f)[DP / (
   }
 }
 
-// 32 LDS rows (plain layout) times a row operand in registers: C rows = the LDS rows, C column = the lane's row
+// 32 LDS rows (plain layout) times a row operand in registers, added to c: C rows = the LDS rows, C column = the lane's row
 template <typename T, int DP>
-__device__ __forceinline__ f32x16 rows_times(const T* s, const typename Elem<T>::vec (&f)[DP / (2 * Elem<T>::kVec)]) {
+__device__ __forceinline__ f32x16 rows_times(const T* s, const typename Elem<T>::vec (&f)[DP / (2 * Elem<T>::kVec)], f32x16 c = {}) {
   constexpr int V = Elem<T>::kVec;
   const int lane = threadIdx.x & 63;
-  f32x16 c = {};
 #pragma unroll
   for (int i = 0; i < DP / (2 * V); ++i)
     Elem<T>::mma(*(const typename Elem<T>::vec*)&s[(lane & 31) * (DP + V) + i * 2 * V + (lane >> 5) * V], f[i], c);
@@ -216,24 +214,38 @@ __device__ __forceinline__ void zero_rows(T* base, long long ld, long long first
   for (long long t = threadIdx.x; t < n; t += blockDim.x) base[(first + t / d) * ld + t % d] = (T)0.f;
 }
 
-// s (fp32 sums) -> log2-unit scores of a 32x32 tile with the keys in the rows and the lane's query as the column, or the
-// other way round; e0 = (first key - first query) of the tile
-template <bool KEYS_IN_ROWS>
-__device__ __forceinline__ void add_bias(f32x16& s, float c, const float* line, int reach, int e0) {
+// Scores in log2 units of a 32x32 tile, the LDS rows s against the lane's row f, with the keys in the rows and the lane's query as the
+// column, or the other way round; e0 = (first key - first query) of the tile.  The same sums in the same order as in the tiled kernels, which
+// may have made the other pass (fp32 heads of 128): the bias is what a tile's sums start from, beyond R it is added behind the product.
+template <typename T, int DP, bool KEYS_IN_ROWS>
+__device__ __forceinline__ f32x16 scores_any(const T* s, const typename Elem<T>::vec (&f)[DP / (2 * Elem<T>::kVec)], float c, const float* line, int reach, int e0, bool even) {
   const int lane = threadIdx.x & 63;
+  f32x16 x;
   if (tile_is_far(e0, reach)) {
-    const float b = line[e0 > 0 ? 2 * reach : 0];
+    const float b = line[e0 > 0 ? 2 * reach : 0], shift = even ? b * c : b;
+    x = rows_times<T, DP>(s, f);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], c, b);      // rounded once in every kernel: see is_great
-    return;
+    for (int r = 0; r < 16; ++r) x[r] = __builtin_fmaf(x[r], c, shift);
+    return x;
   }
+  f32x16 bias;
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
     const int row = (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5), col = lane & 31;
     int e = e0 + (KEYS_IN_ROWS ? row - col : col - row);
     e = e > reach ? reach : e < -reach ? -reach : e;
-    s[r] = __builtin_fmaf(s[r], c, line[reach + e]);
+    bias[r] = line[reach + e];
   }
+  if (even) {
+    x = rows_times<T, DP>(s, f, bias);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] *= c;
+  } else {
+    x = rows_times<T, DP>(s, f);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = __builtin_fmaf(x[r], c, bias[r]);
+  }
+  return x;
 }
 
 // ---- forward, any width, stride and alignment ---------------------------------------------------------------------------
@@ -262,6 +274,7 @@ __global__ __launch_bounds__(NW * 64) void attention_any_kernel(const AttnParams
   typename Elem<T>::vec fq[DP / (2 * V)];
   load_row_frags<T, DP>(fq, (const T*)p.q + (s.begin + i) * p.ld_t + head * p.ld_h, i < len, p.d, p.vec);
   const float c = p.scale * kLog2e;
+  const bool even = even_scale(p.scale);
   float m = -INFINITY, l = 0.f;
   f32x16 acc[DP / 32] = {};
   for (int j0 = 0; j0 < len; j0 += 32) {
@@ -270,8 +283,7 @@ __global__ __launch_bounds__(NW * 64) void attention_any_kernel(const AttnParams
     stage_rows<T, DP, 32, false, true>(nullptr, sv, vb + j0 * p.ld_t, p.ld_t, len - j0, p.d, p.vec, NW * 64);
     __syncthreads();
     if (i0 >= len) continue;
-    f32x16 t = rows_times<T, DP>(sk, fq);
-    add_bias<true>(t, c, line, p.reach, j0 - i0);
+    f32x16 t = scores_any<T, DP, true>(sk, fq, c, line, p.reach, j0 - i0, even);
     if (j0 + 32 > len) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) if (j0 + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5) >= len) t[r] = -INFINITY;
@@ -718,6 +730,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_any_kernel(const AttnPar
   const float delta = i < len ? p.delta[(long long)head * p.total + s.begin + i] : 0.f;
   const float lift = ds_lift<T>(p, head, s.b);
   const float c = p.scale * kLog2e;
+  const bool even = even_scale(p.scale);
   float fix = 0.f;
   if (__builtin_amdgcn_readfirstlane(__syncthreads_or(is_great(lse)))) {
     RowSum row;
@@ -725,8 +738,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_any_kernel(const AttnPar
       __syncthreads();
       stage_rows<T, DP, 32, true, false>(sk, nullptr, kb + j0 * p.ld_t, p.ld_t, len - j0, p.d, p.vec, NW * 64);
       __syncthreads();
-      f32x16 t = rows_times<T, DP>(sk, fq);
-      add_bias<true>(t, c, line, reach, j0 - i0);
+      const f32x16 t = scores_any<T, DP, true>(sk, fq, c, line, reach, j0 - i0, even);
 #pragma unroll
       for (int r = 0; r < 16; ++r) if (j0 + (r & 3) + 8 * (r >> 2) + 4 * half < len) row.add(t[r]);
     }
@@ -742,10 +754,9 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_any_kernel(const AttnPar
     stage_rows<T, DP, 32, true, false>(sv, nullptr, vb + j0 * p.ld_t, p.ld_t, len - j0, p.d, p.vec, NW * 64);
     __syncthreads();
     if (i0 >= len) continue;
-    f32x16 t = rows_times<T, DP>(sk, fq);
-    const f32x16 dp = rows_times<T, DP>(sv, fg);
     const int e0 = j0 - i0;
-    add_bias<true>(t, c, line, reach, e0);
+    f32x16 t = scores_any<T, DP, true>(sk, fq, c, line, reach, e0, even);
+    const f32x16 dp = rows_times<T, DP>(sv, fg);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int j = j0 + (r & 3) + 8 * (r >> 2) + 4 * half;
@@ -807,6 +818,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_any_kernel(const AttnPa
   const float* fix = p.fix + (long long)head * p.total + s.begin;
   const float lift = ds_lift<T>(p, head, s.b), down = lift * kUnlift<T>;
   const float c = p.scale * kLog2e;
+  const bool even = even_scale(p.scale);
   f32x16 ak[DP / 32] = {}, av[DP / 32] = {};
   for (int i0 = 0; i0 < len; i0 += 32) {
     __syncthreads();
@@ -819,9 +831,8 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_any_kernel(const AttnPa
     }
     __syncthreads();
     if (j0 >= len) continue;
-    f32x16 t = rows_times<T, DP>(sq, fk);
+    f32x16 t = scores_any<T, DP, false>(sq, fk, c, line, p.reach, j0 - i0, even);
     const f32x16 dp = rows_times<T, DP>(sg, fv);
-    add_bias<false>(t, c, line, p.reach, j0 - i0);
     f32x16 ds;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
