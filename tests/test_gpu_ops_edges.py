@@ -441,3 +441,20 @@ def test_attention_scores_are_the_same_numbers_forward_and_back(ops, dtype, d):
     v = qkv[:, 2, 0].double()
     assert ((out.detach().cpu()[:, 0].double() - v).abs() <= 4 * ref.E * v.abs()).all()
     assert ((dqkv[:, 2].cpu().double() - dout.double()).abs() <= rel * dout.double().abs() + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [24, 32, 64, 128])
+def test_attention_rows_left_nothing_are_zeros_whatever_v_holds(ops, dtype, d):
+    """All of a head's distances forbidden: zeros, and no gradient, beside infinities and NaN in v."""
+    t, lengths = DT[dtype], [1, 70, 33]
+    g = torch.Generator().manual_seed(d)
+    off = offsets_of(lengths)
+    qkv, table, dout = rnd(g, 104, 3, 2, d, dtype=t), rnd(g, 32, 2, dtype=t), rnd(g, 104, 2, d, dtype=t)
+    table[:, 1] = -math.inf
+    qkv[0, 2, 1, 3], qkv[50, 2, 1, 5], qkv[103, 2, 1, 0] = math.inf, math.nan, -math.inf
+    leaf, tab = qkv.cuda().requires_grad_(), table.cuda().requires_grad_()
+    out = ops.bucketed_attention(leaf, tab, off)
+    dqkv, dtable = torch.autograd.grad(out, [leaf, tab], dout.cuda())
+    assert not out[:, 1].any() and not dqkv[:, :, 1].any() and not dtable[:, 1].any()
+    assert torch.isfinite(out[:, 0]).all() and torch.isfinite(dqkv[:, :, 0]).all()

@@ -70,9 +70,8 @@ __device__ __forceinline__ void make_line(float* line, const AttnParams& p, int 
 // - s is rounded before m is taken away.  Fused, scale x - m keeps the product's exact tail, and half a step of a number like 1e38 is far
 //   beyond any exponent.
 // - The kept lse = m + log2(sum) has no room for log2(sum) there (at the type's lowest value p would be 1 instead of 1 / len): the backward
-//   pass takes such rows' greatest score and sum once more, and keeps the two apart (`from` and `fix`; lse and 0 for other rows).  It takes
-//   both from its own scores: some steps of 1e12 may lie between those and the forward pass' where another kernel made that (fp32
-//   heads of 128).
+//   pass takes such rows' greatest score and sum once more, and keeps the two apart (`from` and `fix`; lse and 0 for other rows).  Both from
+//   its own scores, so that no other kernel's rounding of numbers like 1e12 enters.
 // The tiled kernels do so in a branch ahead of the exponentials that turns a tile's x into (s - m) / c, so that what every tile runs
 // through stays as it is: with a second form of the exponentials in the loop, 16 x 384 tokens in fp32 took 107 us instead of 85.
 __device__ __forceinline__ bool is_great(float x) { return fabsf(x) > 1024.f && fabsf(x) < INFINITY; }
@@ -304,11 +303,16 @@ __global__ __launch_bounds__(NW * 64) void attention_any_kernel(const AttnParams
   }
   if (i >= len) return;
   l += __shfl_xor(l, 32, 64);
-  const float f = l > 0.f || l != l ? 1.f / l : 0.f;
+  const bool left = l > 0.f || l != l;
+  if (!left) {                       // nothing is left of the row: zeros, whatever v holds
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) acc[db] = f32x16{};
+  }
+  const float f = left ? 1.f / l : 0.f;
   store_cols<T, DP>((T*)p.out + (s.begin + i) * hd + (long long)head * p.d, acc, f, p.d, p.vec);
   if (p.rest) store_cols<T, DP, true>((T*)p.rest + (s.begin + i) * hd + (long long)head * p.d, acc, f, p.d, p.vec);
   // +inf where nothing was left of the row: the backward pass' exp2(s - lse) is 0 there
-  if (p.lse && lane < 32) p.lse[(long long)head * p.total + s.begin + i] = l > 0.f || l != l ? m + (log2f(l) - kLift<T>) : INFINITY;
+  if (p.lse && lane < 32) p.lse[(long long)head * p.total + s.begin + i] = left ? m + (log2f(l) - kLift<T>) : INFINITY;
 }
 
 // ---- whole 16-byte pieces and head widths of 32, 64 and 128 ----------------------------------------------------------------
@@ -573,6 +577,10 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams 
   if (i0 >= len) return;
   sum += __shfl_xor(sum, 32, 64);
   const bool any = sum > 0.f || sum != sum;
+  if (!any) {                        // nothing is left of the row: zeros, whatever v holds
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) acc[db] = f32x16{};
+  }
   T* mine = &buf[0][0][0] + wave * (32 * D);
   const float f = any ? 1.f / sum : 0.f;
   store_turned<T, D>(mine, (T*)p.out + (s.begin + i0) * hd + (long long)head * D, hd, acc, f, len - i0);
