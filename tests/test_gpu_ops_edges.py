@@ -458,3 +458,22 @@ def test_attention_rows_left_nothing_are_zeros_whatever_v_holds(ops, dtype, d):
     dqkv, dtable = torch.autograd.grad(out, [leaf, tab], dout.cuda())
     assert not out[:, 1].any() and not dqkv[:, :, 1].any() and not dtable[:, 1].any()
     assert torch.isfinite(out[:, 0]).all() and torch.isfinite(dqkv[:, :, 0]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [24, 32, 64, 128])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_attention_gradients_know_no_bucket_that_the_text_does_not_meet(ops, dtype, d, value):
+    """NaN or +inf in the buckets of distances from 8 on: texts of at most 8 tokens have the gradients that they have without."""
+    t, lengths = DT[dtype], [1, 8, 5, 1, 7]
+    g = torch.Generator().manual_seed(d)
+    off = offsets_of(lengths)
+    qkv, table, dout = rnd(g, 22, 3, 2, d, dtype=t).cuda(), rnd(g, 32, 2, dtype=t).cuda(), rnd(g, 22, 2, d, dtype=t).cuda()
+    bad = table.clone()
+    bad[8:16], bad[24:] = value, value
+    grads = []
+    for tab in (table, bad):
+        leaf, tab = qkv.clone().requires_grad_(), tab.clone().requires_grad_()
+        out = ops.bucketed_attention(leaf, tab, off)
+        grads.append([out.detach(), *torch.autograd.grad(out, [leaf, tab], dout)])
+    assert all(torch.equal(a, b) for a, b in zip(*grads))

@@ -768,7 +768,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_any_kernel(const AttnPar
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int j = j0 + (r & 3) + 8 * (r >> 2) + 4 * half;
-      const float w = j < len ? __builtin_amdgcn_exp2f(t[r] - lse - fix) : 0.f;
+      const float w = j < len && i < len ? __builtin_amdgcn_exp2f(t[r] - lse - fix) : 0.f;      // what is not there meets any bias
       t[r] = w == 0.f ? 0.f : w * (dp[r] - delta);
     }
     if constexpr (DTABLE) {
@@ -845,7 +845,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dkv_any_kernel(const AttnPa
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int row = (r & 3) + 8 * (r >> 2) + 4 * half;
-      t[r] = __builtin_amdgcn_exp2f(t[r] - sl[row] - sf[row] + kLift<T>);
+      t[r] = i0 + row < len ? __builtin_amdgcn_exp2f(t[r] - sl[row] - sf[row] + kLift<T>) : 0.f;      // a query that is not there meets any bias
       ds[r] = t[r] == 0.f ? 0.f : t[r] * (dp[r] - sd[row]);
     }
     trans_times<T, DP>(av, sgt, t);
@@ -1051,6 +1051,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
 #pragma unroll
         for (int r = 0; r < 16; ++r) if (j0 + (r & 3) + 8 * (r >> 2) + 4 * half >= len) x[r] = 0.f;
       }
+      if (i0 + 32 > len && i0 + l >= len) x = f32x16{};       // a query that is not there meets any bias, NaN and infinities too
       if constexpr (DTABLE) {
         if (is_far) {
           float y = 0.f;
@@ -1176,6 +1177,10 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
           x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], c, shift - ls[e]));
           dp[r] = x[r] == 0.f ? 0.f : x[r] * (dp[r] - dl[e]);       // a forbidden place may hold anything
         }
+      }
+      if (t * QT + u * 32 + 32 > len) {      // a query that is not there meets any bias, NaN and infinities too
+#pragma unroll
+        for (int r = 0; r < 16; ++r) if (t * QT + u * 32 + (r & 3) + 8 * (r >> 2) + 4 * half >= len) x[r] = dp[r] = 0.f;
       }
       add_across<T, D>(av, sg, u * 32, x);
       if (down != 1.f) dp *= down;
