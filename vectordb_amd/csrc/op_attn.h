@@ -70,7 +70,7 @@ __device__ __forceinline__ void make_line(float* line, const AttnParams& p, int 
 // - s is rounded before m is taken away.  Fused, scale x - m keeps the product's exact tail, and half a step of a number like 1e38 is far
 //   beyond any exponent.
 // - The kept lse = m + log2(sum) has no room for log2(sum) there (at the type's lowest value p would be 1 instead of 1 / len): the backward
-//   pass takes such rows' greatest score and sum once more, and keeps the two apart (`from` and `fix`; lse and 0 for other rows).  Both from
+//   pass takes such rows' greatest score and sum once more, and keeps the two apart (`from` and `fix`, which is never 0; lse and 0 for other rows).  Both from
 //   its own scores, so that no other kernel's rounding of numbers like 1e12 enters.
 // The tiled kernels do so in a branch ahead of the exponentials that turns a tile's x into (s - m) / c, so that what every tile runs
 // through stays as it is: with a second form of the exponentials in the loop, 16 x 384 tokens in fp32 took 107 us instead of 85.
@@ -392,14 +392,15 @@ __device__ __forceinline__ void add_across(f32x16 (&acc)[D / 32], const T* s, in
 
 // line[start_at(R, e)] = bias(e) / scale, |e| <= R + kMargin: the start value of a tile's sums, so that a tile near the diagonal costs a
 // look-up a score and no arithmetic.  Only the distances that a text of this length meets are filled in (around: its length and
-// a tile; a far tile, which takes its bias from an end of the line, is met only where all of it is).
-template <typename T>
-__device__ __forceinline__ void make_start_line(float* line, const AttnParams& p, int head, float c, int around) {
+// a tile; a far tile, which takes its bias from an end of the line, is met only where all of it is).  VOTE: -> whether any thread says so.
+template <typename T, bool VOTE = false>
+__device__ __forceinline__ bool make_start_line(float* line, const AttnParams& p, int head, float c, int around, bool vote = false) {
   __shared__ float tab[128];
   for (int t = threadIdx.x; t < p.n_buckets; t += blockDim.x) tab[t] = start_value((float)((const T*)p.table)[(long long)t * p.heads + head], p.scale, c);
-  __syncthreads();
+  if constexpr (VOTE) vote = __builtin_amdgcn_readfirstlane(__syncthreads_or(vote)); else __syncthreads();
   const int middle = start_zero(p.reach), w = around < middle ? around : middle;
   for (int t = middle - w + threadIdx.x; t <= middle + w; t += blockDim.x) line[t] = tab[bucket_of(p.bk, t - middle)];
+  return vote;
 }
 
 // Waits for what the compiler has loaded into x, here: left to itself it waits where x is used first, inside the loop over tiles, and
@@ -553,11 +554,12 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kernel(const AttnParams 
 #pragma unroll
       for (int db = 0; db < D / 32; ++db) acc[db] *= fade;
       great = __any(is_great(m));
-      if (great) {
+      if (__builtin_expect(great, 0)) {
+        const float back = 1.f / c;
 #pragma unroll
         for (int u = 0; u < KT / 32; ++u) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) x[u][r] = (__builtin_fmaf(x[u][r], c, shift[u]) - base + kLift<T>) / c;
+          for (int r = 0; r < 16; ++r) x[u][r] = (__builtin_fmaf(x[u][r], c, shift[u]) - base + kLift<T>) * back;
           shift[u] = 0.f;
         }
         base = kLift<T>;
@@ -751,7 +753,7 @@ __global__ __launch_bounds__(NW * 64) void attention_dq_any_kernel(const AttnPar
       for (int r = 0; r < 16; ++r) if (j0 + (r & 3) + 8 * (r >> 2) + 4 * half < len) row.add(t[r]);
     }
     row.join();
-    if (is_great(lse)) { lse = row.top; fix = log2f(row.sum); }
+    if (is_great(lse)) { lse = row.top; fix = log2f(row.sum) + 1e-30f; }
   }
   if (lane < 32 && i < len) { p.from[(long long)head * p.total + s.begin + i] = lse; p.fix[(long long)head * p.total + s.begin + i] = fix; }
   float below = 0.f, above = 0.f;
@@ -981,7 +983,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
   const float lift = ds_lift<T>(p, head, s.b);
   const float c = p.scale * kLog2e;
   float* hist = line + start_span(reach);
-  make_start_line<T>(line, p, head, c, len + KT);
+  const bool great = make_start_line<T, true>(line, p, head, c, len + KT, is_great(lse));
   if constexpr (DTABLE) for (int t = threadIdx.x; t < NW * 2 * span; t += NW * 64) hist[t] = 0.f;
   const float* mid = line + start_at(reach, 4 * half - l);
   float* mine = hist + (wave * 2 + half) * span;
@@ -991,8 +993,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
   settle(lse);
   settle(less);
   float fix = 0.f;
-  const bool great = __builtin_amdgcn_readfirstlane(__syncthreads_or(is_great(lse)));
-  if (great) {
+  if (__builtin_expect(great, 0)) {
     RowSum all;
     for (int t = 0; t < tiles; ++t) {
       wait_loads<0>();
@@ -1011,12 +1012,13 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
       }
     }
     all.join();
-    if (is_great(lse)) { lse = all.top; fix = log2f(all.sum); }
+    if (is_great(lse)) { lse = all.top; fix = log2f(all.sum) + 1e-30f; }
     __syncthreads();                 // the last tile is read: its place may be loaded again
     issue(0);
   }
   if (lane < 32 && i0 + l < len) { p.from[row] = lse; p.fix[row] = fix; }
   const float from = -lse;
+  const bool seldom = great || __builtin_amdgcn_readfirstlane(i0 + 32 > len);
   float below = 0.f, above = 0.f;
   f32x16 acc[D / 32] = {};
   for (int t = 0; t < tiles; ++t) {
@@ -1033,15 +1035,20 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
       const bool is_far = tile_is_far(e0, reach);
       f32x16 x, dp = {};
       float shift = c * scores<T, D, R, 1>(x, sk, u * 32, fq, e0, p, line, mid + e0);
-      if (great) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] = (__builtin_fmaf(x[r], c, shift) + from - fix) / c;
-        shift = 0.f;
-      } else {
-        shift += from;
-      }
 #pragma unroll
       for (int y = 0; y < D / (2 * V); ++y) Elem<T>::mma(RV::along(sv, u * 32, y), fg[y], dp);
+      if (__builtin_expect(seldom, 0)) {
+        if (i0 + l >= len) {           // a query that is not there meets any bias, NaN and infinities too
+#pragma unroll
+          for (int r = 0; r < 16; ++r) x[r] = -INFINITY;
+        }
+        if (great) {
+          const float back = 1.f / c;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) x[r] = (__builtin_fmaf(x[r], c, shift) + from - fix) * back;
+        }
+      }
+      shift = great ? 0.f : shift + from;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], c, shift));
@@ -1051,7 +1058,6 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
 #pragma unroll
         for (int r = 0; r < 16; ++r) if (j0 + (r & 3) + 8 * (r >> 2) + 4 * half >= len) x[r] = 0.f;
       }
-      if (i0 + 32 > len && i0 + l >= len) x = f32x16{};       // a query that is not there meets any bias, NaN and infinities too
       if constexpr (DTABLE) {
         if (is_far) {
           float y = 0.f;
@@ -1084,8 +1090,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
   using R = Rows<T, D, kCol>;
   using vec = typename Elem<T>::vec;
   __shared__ __align__(1024) T buf[2][2][QT * D];       // [turn][q, dout]
-  __shared__ __align__(16) float stat[2][4][QT];             // [turn][lse (a great tile: 0), delta, a great tile: lse, fix]
-  __shared__ int some_great[2];                              // [turn]: whether any of the tile's queries is
+  __shared__ __align__(16) float stat[2][4][QT];             // [turn][lse, delta]; a text with great rows: [0, delta, lse, fix]
   extern __shared__ float line[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l = lane & 31;
   int head;
@@ -1106,7 +1111,8 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
   const float* lse = p.from + (long long)head * p.total + s.begin;
   const float* delta = p.delta + (long long)head * p.total + s.begin;
   const float* fix = p.fix + (long long)head * p.total + s.begin;
-  float next_lse = 0.f, next_delta = 0.f, next_fix = 0.f;    // thread x < QT, the first wave: of query x of the tile under way
+  float next_lse = 0.f, next_delta = 0.f, next_fix = 0.f;    // thread x < QT: of query x of the tile under way
+  bool great = false;                        // some query of the text has a fix
   auto issue = [&](int t) {
     const int left = len - t * QT;
     R::template load<QT, NW * 64>(buf[t & 1][0], qb + (long long)t * QT * p.ld_t, p.ld_t, left);
@@ -1115,7 +1121,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
       const bool there = (int)threadIdx.x < left;
       next_lse = there ? lse[t * QT + threadIdx.x] : INFINITY;
       next_delta = there ? delta[t * QT + threadIdx.x] : 0.f;
-      next_fix = there ? fix[t * QT + threadIdx.x] : 0.f;
+      next_fix = great && there ? fix[t * QT + threadIdx.x] : 0.f;
     }
   };
   issue(0);
@@ -1129,19 +1135,19 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
   }
   const float lift = ds_lift<T>(p, head, s.b), down = lift * kUnlift<T>;
   const float c = p.scale * kLog2e;
-  make_start_line<T>(line, p, head, c, len + QT);
+#pragma unroll 4
+  for (int i = threadIdx.x; i < len; i += NW * 64) great |= fix[i] != 0.f;
+  great = make_start_line<T, true>(line, p, head, c, len + QT, great);
+  if (great && threadIdx.x < QT) next_fix = (int)threadIdx.x < len ? fix[threadIdx.x] : 0.f;
   const float* mid = line + start_at(p.reach, l - 4 * half);        // mid[e0 - row]: column l is the key, the rows are queries
 #pragma unroll
   for (int x = 0; x < D / (2 * V); ++x) { settle(fk[x]); settle(fv[x]); }
   f32x16 ak[D / 32] = {}, av[D / 32] = {};
   for (int t = 0; t < tiles; ++t) {
     if (threadIdx.x < QT) {
-      const bool any = __any(is_great(next_lse) || next_fix != 0.f);
-      stat[t & 1][0][threadIdx.x] = any ? 0.f : next_lse;
+      stat[t & 1][0][threadIdx.x] = great ? 0.f : next_lse;
       stat[t & 1][1][threadIdx.x] = next_delta;
-      stat[t & 1][2][threadIdx.x] = next_lse;
-      stat[t & 1][3][threadIdx.x] = next_fix;
-      if (threadIdx.x == 0) some_great[t & 1] = any;
+      if (great) { stat[t & 1][2][threadIdx.x] = next_lse; stat[t & 1][3][threadIdx.x] = next_fix; }
     }
     wait_loads<0>();
     __syncthreads();
@@ -1149,25 +1155,23 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
     if (j0 >= len) continue;
     const T* sq = buf[t & 1][0];
     const T* sg = buf[t & 1][1];
-    const bool great = __builtin_amdgcn_readfirstlane(some_great[t & 1]);
 #pragma unroll 1
     for (int u = 0; u < QT / 32; ++u) {
       if (t * QT + u * 32 >= len) break;
       const int e0 = j0 - t * QT - u * 32;
       f32x16 x, dp = {};
       float shift = c * scores<T, D, R, -1>(x, sq, u * 32, fk, e0, p, line, mid + e0);
-      if (great) {
+#pragma unroll
+      for (int y = 0; y < D / (2 * V); ++y) Elem<T>::mma(R::along(sg, u * 32, y), fv[y], dp);
+      if (__builtin_expect(great || t * QT + u * 32 + 32 > len, 0)) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int row = u * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
-          x[r] = (__builtin_fmaf(x[r], c, shift) - stat[t & 1][2][row] - stat[t & 1][3][row] + kLift<T>) / c;
+          if (great) x[r] = (__builtin_fmaf(x[r], c, shift) - stat[t & 1][2][row] - stat[t & 1][3][row] + kLift<T>) * (1.f / c);
+          if (t * QT + row >= len) x[r] = -INFINITY;       // a query that is not there meets any bias, NaN and infinities too
         }
-        shift = 0.f;
-      } else {
-        shift += kLift<T>;
       }
-#pragma unroll
-      for (int y = 0; y < D / (2 * V); ++y) Elem<T>::mma(R::along(sg, u * 32, y), fv[y], dp);
+      shift = great ? 0.f : shift + kLift<T>;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const f32x4 ls = *(const f32x4*)&stat[t & 1][0][u * 32 + 8 * g + 4 * half], dl = *(const f32x4*)&stat[t & 1][1][u * 32 + 8 * g + 4 * half];
@@ -1177,10 +1181,6 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kerne
           x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], c, shift - ls[e]));
           dp[r] = x[r] == 0.f ? 0.f : x[r] * (dp[r] - dl[e]);       // a forbidden place may hold anything
         }
-      }
-      if (t * QT + u * 32 + 32 > len) {      // a query that is not there meets any bias, NaN and infinities too
-#pragma unroll
-        for (int r = 0; r < 16; ++r) if (t * QT + u * 32 + (r & 3) + 8 * (r >> 2) + 4 * half >= len) x[r] = dp[r] = 0.f;
       }
       add_across<T, D>(av, sg, u * 32, x);
       if (down != 1.f) dp *= down;
