@@ -920,7 +920,7 @@ __device__ __forceinline__ Slot place_of(const AttnParams& p, unsigned slots, un
 
 // dq and the block's bucket sums.  Each wave: 32 queries, one per lane column; key tiles of 64 through LDS.  k is read along its
 // rows (scores) and across them (ds k): one copy in LDS, in the order of the transposed reads, serves both - the reads along it
-// meet two by two on a bank.  64 texts of 16 to 384 tokens, 12 heads of 64, bf16: 52 us, 0.30 PFLOP/s, 19 vector instructions a
+// meet two by two on a bank.  64 texts of 16 to 384 tokens, 12 heads of 64, bf16: 53 us, 0.30 PFLOP/s, 19 vector instructions a
 // score: bound by their issue and by the latency of a chain a tile.
 template <typename T, int D, int NW, bool DTABLE>
 __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel(const AttnParams p, unsigned slots, unsigned hop) {
@@ -1083,7 +1083,7 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dq_kernel
 
 // dk and dv: each wave 32 keys, one per lane column; query tiles of 64 through LDS, q and dout once, in the order of the
 // transposed reads.  The two halves of a tile one after the other: held together they cost registers, 63 us
-// instead of 58 at the size above, 54 with the longest texts first (0.38 PFLOP/s).
+// instead of 58 at the size above, 52 with the longest texts first, 58 with what great rows and absent places need (0.35 PFLOP/s).
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void attention_dkv_kernel(const AttnParams p, unsigned slots, unsigned hop) {
   constexpr int BQ = NW * 32, QT = 64, V = Elem<T>::kVec;
